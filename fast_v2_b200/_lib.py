@@ -38,6 +38,12 @@ EXPORTS = (
     "fdl_focus_select",
     "fdl_focus_importance",
     "fdl_softmax_argmax",
+    "fdl_page_slots",
+    "fdl_page_release",
+    "fdl_norm_rope_store",
+    "fdl_paged_attn_workspace_bytes",
+    "fdl_paged_attn",
+    "fdl_token_logprobs",
     "fdl_last_device_error",
     "fdl_version",
 )
@@ -78,6 +84,8 @@ def abi() -> ctypes.CDLL:
             lib.fdl_block_attn_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
             lib.fdl_block_attn_auto_splits.restype = i32
             lib.fdl_block_attn_auto_splits.argtypes = [i32] * 6
+            lib.fdl_paged_attn_workspace_bytes.restype = i64
+            lib.fdl_paged_attn_workspace_bytes.argtypes = [i32, i32, i32, i32, i64]
             lib.fdl_last_device_error.restype = i32
             lib.fdl_last_device_error.argtypes = [ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(i64)]
             del vp

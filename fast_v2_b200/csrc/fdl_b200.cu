@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <initializer_list>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv_copy.cuh"
@@ -14,6 +15,10 @@
 #include "rope_swiglu.cuh"
 #include "token_select.cuh"
 #include "sampling.cuh"
+#include "page_slots.cuh"
+#include "norm_rope.cuh"
+#include "paged_attn.cuh"
+#include "token_scores.cuh"
 
 using namespace fdl;
 
@@ -711,6 +716,142 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows, int voc
   SampleArgs a{static_cast<const __nv_bfloat16*>(logits), row_stride, vocab, token,
                static_cast<__nv_bfloat16*>(prob)};
   softmax_argmax_kernel<<<static_cast<unsigned>(rows), kSampleThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  return launch_status();
+}
+
+int fdl_page_slots(const int32_t* lens, const int32_t* n_new, int batch, int32_t* table, int64_t table_sb,
+                   int max_pages, const int32_t* free_pages, int n_free, int32_t* count, int page_size, int64_t* slots,
+                   int64_t* positions, int64_t n_rows, int32_t* cu, int32_t* new_lens, int32_t* new_count,
+                   fdl_stream_t stream) {
+  if (batch < 1 || batch > kSlotsMaxBatch || max_pages < 0 || n_free < 0 || page_size < 1 || n_rows < 0 ||
+      n_rows > INT32_MAX || table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+    return FDL_E_SHAPE;
+  if (!lens || !n_new || !count || !cu || !new_lens || !new_count || (max_pages > 0 && !table) ||
+      (n_free > 0 && !free_pages) || (n_rows > 0 && (!slots || !positions)))
+    return FDL_E_NULL;
+  PageSlotsArgs a{lens, n_new, table, table_sb, free_pages, count, slots, positions, cu, new_lens, new_count,
+                  batch, max_pages, n_free, {}, n_rows};
+  a.page.init(static_cast<uint32_t>(page_size));
+  const int grid = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(num_sms(), (n_rows + kSlotsThreads - 1) / kSlotsThreads)));
+  page_slots_kernel<<<grid, kSlotsThreads, (2 * batch + 1) * sizeof(int32_t), reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  return launch_status();
+}
+
+int fdl_page_release(const uint8_t* done, int32_t* lens, int batch, int32_t* table, int64_t table_sb, int max_pages,
+                     int32_t* free_pages, int n_free, int32_t* count, int page_size, fdl_stream_t stream) {
+  if (batch < 1 || batch > kSlotsMaxBatch || max_pages < 0 || n_free < 0 || page_size < 1 || table_sb < max_pages ||
+      static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+    return FDL_E_SHAPE;
+  if (!done || !lens || !count || (max_pages > 0 && !table) || (n_free > 0 && !free_pages)) return FDL_E_NULL;
+  PageReleaseArgs a{done, lens, table, table_sb, free_pages, count, batch, max_pages, n_free, {}};
+  a.page.init(static_cast<uint32_t>(page_size));
+  page_release_kernel<<<1, kSlotsThreads, batch * sizeof(int32_t), reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  return launch_status();
+}
+
+int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos, const float* inv_freq, int n_freq,
+                        const void* q_weight, const void* k_weight, float eps, int interleaved, float rope_scale,
+                        void* q, void* k_pages, void* v_pages, int64_t kv_sp, int64_t kv_ss, int64_t kv_sh,
+                        int num_pages, int page_size, const int64_t* slots, int64_t rows, int hq, int hkv,
+                        int head_dim, int dtype, fdl_stream_t stream) {
+  if (dtype != FDL_BF16 && dtype != FDL_F16) return FDL_E_DTYPE;
+  if (rows < 0 || rows > INT32_MAX || hq < 1 || hkv < 1 || head_dim < 16 || head_dim % 16 ||
+      head_dim > kNrMaxDim || n_freq < 0 || n_freq % 8 || 2 * n_freq > head_dim || num_pages < 1 || page_size < 1 ||
+      static_cast<int64_t>(num_pages) * page_size > INT32_MAX)
+    return FDL_E_SHAPE;
+  const int64_t width = (static_cast<int64_t>(hq) + 2 * static_cast<int64_t>(hkv)) * head_dim;
+  if (width > (1 << 24) || (rows > 1 && y_rs < width)) return FDL_E_SHAPE;
+  if (rows == 0) return FDL_OK;
+  if (!y || !pos || (n_freq > 0 && !inv_freq) || !q || !k_pages || !v_pages || !slots) return FDL_E_NULL;
+  for (const void* p : {y, static_cast<const void*>(q), static_cast<const void*>(k_pages),
+                        static_cast<const void*>(v_pages), q_weight, k_weight})
+    if (!aligned16(p)) return FDL_E_ALIGN;
+  for (int64_t st : {y_rs, kv_sp, kv_ss, kv_sh})
+    if ((st * 2) % 16) return FDL_E_ALIGN;
+  NormRopeArgs a{y, y_rs, pos, inv_freq, q_weight, k_weight, q, static_cast<char*>(k_pages),
+                 static_cast<char*>(v_pages), kv_sp * 2, kv_ss * 2, kv_sh * 2, slots,
+                 static_cast<int64_t>(num_pages) * page_size, {}, eps, rope_scale, static_cast<int>(rows), hq, hkv,
+                 head_dim, 2 * n_freq};
+  a.page.init(static_cast<uint32_t>(page_size));
+  int gs = 1;
+  while (gs * 16 < head_dim) gs *= 2;
+  const int64_t lanes = (static_cast<int64_t>(hq) + 2 * static_cast<int64_t>(hkv)) * gs;
+  const int threads = static_cast<int>(std::min<int64_t>(kNrMaxThreads, (lanes + 31) / 32 * 32));
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) {
+    kernel<<<static_cast<unsigned>(rows), threads, 0, s>>>(a);
+    return launch_status();
+  };
+  auto by_gs = [&](auto t, auto inter) {
+    using T = decltype(t);
+    constexpr bool kInter = decltype(inter)::value;
+    switch (gs) {
+      case 1: return go(norm_rope_kernel<T, 1, kInter>);
+      case 2: return go(norm_rope_kernel<T, 2, kInter>);
+      case 4: return go(norm_rope_kernel<T, 4, kInter>);
+      case 8: return go(norm_rope_kernel<T, 8, kInter>);
+      default: return go(norm_rope_kernel<T, 16, kInter>);
+    }
+  };
+  if (dtype == FDL_BF16)
+    return interleaved ? by_gs(__nv_bfloat16{}, std::true_type{}) : by_gs(__nv_bfloat16{}, std::false_type{});
+  return interleaved ? by_gs(__half{}, std::true_type{}) : by_gs(__half{}, std::false_type{});
+}
+
+int64_t fdl_paged_attn_workspace_bytes(int batch, int hq, int hkv, int head_dim, int64_t max_len) {
+  (void)batch; (void)hq; (void)hkv; (void)head_dim; (void)max_len;
+  return 0;
+}
+
+int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages, int64_t kv_sp,
+                   int64_t kv_ss, int64_t kv_sh, int num_pages, int page_size, const int32_t* table, int64_t table_sb,
+                   int max_pages, const int32_t* lens, int batch, int hq, int hkv, int head_dim, int dtype, float scale,
+                   void* out, int64_t o_sb, int64_t o_sh, void* workspace, int64_t workspace_bytes,
+                   fdl_stream_t stream) {
+  if (dtype != FDL_BF16 && dtype != FDL_F16) return FDL_E_DTYPE;
+  if (batch < 0 || batch > 65535 || hq < 1 || hkv < 1 || hq % hkv || num_pages < 0 || page_size < 1 || max_pages < 0 ||
+      table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+    return FDL_E_SHAPE;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FDL_E_UNSUPPORTED;
+  if (batch == 0) return FDL_OK;
+  if (!q || !lens || !out || (max_pages > 0 && !table) || (num_pages > 0 && (!k_pages || !v_pages))) return FDL_E_NULL;
+  for (const void* p : {q, k_pages, v_pages, static_cast<const void*>(out)})
+    if (!aligned16(p)) return FDL_E_ALIGN;
+  for (int64_t st : {q_sb, q_sh, kv_sp, kv_ss, kv_sh, o_sb, o_sh})
+    if ((st * 2) % 16) return FDL_E_ALIGN;
+  (void)workspace; (void)workspace_bytes;
+  PagedAttnArgs a{q, q_sb, q_sh, static_cast<const char*>(k_pages), static_cast<const char*>(v_pages), kv_sp * 2,
+                  kv_ss * 2, kv_sh * 2, table, table_sb, lens, out, o_sb, o_sh, batch, hq, hkv, num_pages, max_pages,
+                  {}, scale * 1.4426950408889634f};
+  a.page.init(static_cast<uint32_t>(page_size));
+  const dim3 grid(hq, batch);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) {
+    kernel<<<grid, kPagedThreads, 0, s>>>(a);
+    return launch_status();
+  };
+  auto by_d = [&](auto t) {
+    using T = decltype(t);
+    return head_dim == 64 ? go(paged_attn_kernel<T, 64>)
+                          : head_dim == 128 ? go(paged_attn_kernel<T, 128>) : go(paged_attn_kernel<T, 256>);
+  };
+  return dtype == FDL_BF16 ? by_d(__nv_bfloat16{}) : by_d(__half{});
+}
+
+int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int vocab, int dtype, const int64_t* targets,
+                       float* logprob, float* entropy, int top, float* top_logprob, int64_t* top_token,
+                       fdl_stream_t stream) {
+  if (dtype != FDL_BF16 && dtype != FDL_F16 && dtype != FDL_F32) return FDL_E_DTYPE;
+  if (rows < 0 || vocab < 1 || row_stride < vocab || top < 0 || top > kTokMaxTop || top > vocab) return FDL_E_SHAPE;
+  if (rows == 0) return FDL_OK;
+  if (!logits || !targets || !logprob || !entropy || (top > 0 && (!top_logprob || !top_token))) return FDL_E_NULL;
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == FDL_F32 ? 4 : 2)) return FDL_E_ALIGN;
+  TokScoreArgs a{logits, row_stride, vocab, targets, logprob, entropy, top, top_logprob, top_token};
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == FDL_BF16) token_scores_kernel<__nv_bfloat16><<<rows, kTokThreads, 0, s>>>(a);
+  else if (dtype == FDL_F16) token_scores_kernel<__half><<<rows, kTokThreads, 0, s>>>(a);
+  else token_scores_kernel<float><<<rows, kTokThreads, 0, s>>>(a);
   return launch_status();
 }
 

@@ -620,6 +620,191 @@ void add_rmsnorm(const Tensor& x, const Tensor& res, const std::optional<Tensor>
            "add_rmsnorm");
 }
 
+// ---------------------------------------------------------------- paged cache
+void check_i32(const Tensor& t, const Tensor& like, int64_t n, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous() &&
+                  t.numel() == n,
+              "fdl: ", what, " must be a contiguous int32 tensor of ", n, " entries on ", like.device());
+}
+
+void check_i64(const Tensor& t, const Tensor& like, int64_t n, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kLong && t.is_contiguous() &&
+                  t.numel() == n,
+              "fdl: ", what, " must be a contiguous int64 tensor of ", n, " entries on ", like.device());
+}
+
+void check_table(const Tensor& table, const Tensor& like, int64_t B) {
+  TORCH_CHECK(table.is_cuda() && table.device() == like.device() && table.scalar_type() == at::kInt &&
+                  table.dim() == 2 && table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1) &&
+                  (B <= 1 || table.stride(0) >= table.size(1)),
+              "fdl: block_table must be an int32 [", B, ", max_pages] tensor with unit inner stride on ",
+              like.device());
+}
+
+int64_t table_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// Sizes that the C ABI takes as int.
+int as_int(int64_t v, const char* what) {
+  TORCH_CHECK(v >= 0 && v <= INT32_MAX, "fdl: ", what, " is ", v, ", outside [0, 2^31)");
+  return static_cast<int>(v);
+}
+
+void check_pool(const Tensor& lens, const Tensor& free_pages, const Tensor& free_count) {
+  TORCH_CHECK(lens.is_cuda() && lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.is_contiguous(),
+              "fdl: lens must be a contiguous CUDA int32 [B] tensor");
+  check_i32(free_pages, lens, free_pages.numel(), "free_pages");
+  check_i32(free_count, lens, 2, "free_count");
+}
+
+void page_slots(const Tensor& lens, const Tensor& n_new, const Tensor& block_table, const Tensor& free_pages,
+                const Tensor& free_count, int64_t page_size, const Tensor& slots, const Tensor& positions,
+                const Tensor& cu_seqlens, const std::optional<Tensor>& new_lens,
+                const std::optional<Tensor>& new_count) {
+  check_pool(lens, free_pages, free_count);
+  const int64_t B = lens.numel();
+  check_i32(n_new, lens, B, "n_new");
+  check_table(block_table, lens, B);
+  check_i64(slots, lens, slots.numel(), "slots");
+  check_i64(positions, lens, slots.numel(), "positions");
+  check_i32(cu_seqlens, lens, B + 1, "cu_seqlens");
+  if (new_lens) check_i32(*new_lens, lens, B, "new_lens");
+  if (new_count) check_i32(*new_count, lens, 2, "new_count");
+  TORCH_CHECK(page_size >= 1, "fdl.page_slots: page_size is ", page_size);
+  c10::cuda::CUDAGuard guard(lens.device());
+  check_rc(fdl_page_slots(lens.data_ptr<int32_t>(), n_new.data_ptr<int32_t>(), as_int(B, "the batch"),
+                          block_table.data_ptr<int32_t>(), table_stride(block_table),
+                          as_int(block_table.size(1), "max_pages"), free_pages.data_ptr<int32_t>(),
+                          as_int(free_pages.numel(), "the pool"), free_count.data_ptr<int32_t>(),
+                          as_int(page_size, "page_size"), slots.data_ptr<int64_t>(), positions.data_ptr<int64_t>(),
+                          slots.numel(), cu_seqlens.data_ptr<int32_t>(),
+                          new_lens ? new_lens->data_ptr<int32_t>() : lens.data_ptr<int32_t>(),
+                          new_count ? new_count->data_ptr<int32_t>() : free_count.data_ptr<int32_t>(), cur_stream()),
+           "page_slots");
+}
+
+void page_release(const Tensor& done, const Tensor& lens, const Tensor& block_table, const Tensor& free_pages,
+                  const Tensor& free_count, int64_t page_size) {
+  check_pool(lens, free_pages, free_count);
+  const int64_t B = lens.numel();
+  TORCH_CHECK(done.is_cuda() && done.device() == lens.device() && done.scalar_type() == at::kBool &&
+                  done.is_contiguous() && done.numel() == B,
+              "fdl.page_release: done must be a contiguous bool [", B, "] tensor on ", lens.device());
+  check_table(block_table, lens, B);
+  TORCH_CHECK(page_size >= 1, "fdl.page_release: page_size is ", page_size);
+  c10::cuda::CUDAGuard guard(lens.device());
+  check_rc(fdl_page_release(reinterpret_cast<const uint8_t*>(done.data_ptr()), lens.data_ptr<int32_t>(),
+                            as_int(B, "the batch"), block_table.data_ptr<int32_t>(), table_stride(block_table),
+                            as_int(block_table.size(1), "max_pages"), free_pages.data_ptr<int32_t>(),
+                            as_int(free_pages.numel(), "the pool"), free_count.data_ptr<int32_t>(),
+                            as_int(page_size, "page_size"), cur_stream()),
+           "page_release");
+}
+
+// K and V pages [num_pages, page_size, Hkv, D], one layout for both.
+void check_pages(const Tensor& k, const Tensor& v, const Tensor& like, const char* op) {
+  TORCH_CHECK(k.is_cuda() && k.device() == like.device() && v.device() == like.device() && k.dim() == 4 &&
+                  k.dtype() == like.dtype() && v.dtype() == like.dtype() && v.sizes() == k.sizes() &&
+                  v.strides() == k.strides() && k.stride(3) == 1,
+              "fdl.", op, ": k_pages and v_pages must be [num_pages, page_size, Hkv, D] tensors of one layout, of ",
+              like.dtype(), " on ", like.device(), ", contiguous in D");
+}
+
+void norm_rope_store(const Tensor& y, const Tensor& positions, const Tensor& inv_freq,
+                     const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight, double eps,
+                     bool interleaved, double rope_scale, const Tensor& q, const Tensor& k_pages,
+                     const Tensor& v_pages, const Tensor& slots) {
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && y.stride(1) == 1,
+              "fdl.norm_rope_store: y must be a CUDA [rows, (hq + 2 hkv) * D] tensor with unit inner stride");
+  TORCH_CHECK(q.is_cuda() && q.device() == y.device() && q.dtype() == y.dtype() && q.dim() == 3 && q.is_contiguous() &&
+                  q.size(0) == y.size(0),
+              "fdl.norm_rope_store: q must be a contiguous [rows, hq, D] tensor of y's type on its device");
+  check_pages(k_pages, v_pages, y, "norm_rope_store");
+  const int64_t rows = y.size(0), hq = q.size(1), D = q.size(2), hkv = k_pages.size(2);
+  TORCH_CHECK(k_pages.size(3) == D && y.size(1) == (hq + 2 * hkv) * D, "fdl.norm_rope_store: y ", y.sizes(), ", q ",
+              q.sizes(), " and pages ", k_pages.sizes(), " do not fit together");
+  check_i64(positions, y, rows, "positions");
+  check_i64(slots, y, rows, "slots");
+  TORCH_CHECK(inv_freq.is_cuda() && inv_freq.device() == y.device() && inv_freq.scalar_type() == at::kFloat &&
+                  inv_freq.dim() == 1 && inv_freq.is_contiguous(),
+              "fdl.norm_rope_store: inv_freq must be a contiguous fp32 tensor on ", y.device());
+  for (const auto* w : {&q_weight, &k_weight})
+    if (*w)
+      TORCH_CHECK((*w)->is_cuda() && (*w)->device() == y.device() && (*w)->dtype() == y.dtype() && (*w)->dim() == 1 &&
+                      (*w)->numel() == D && (*w)->is_contiguous(),
+                  "fdl.norm_rope_store: head norm weights must be contiguous [D] tensors of y's type on ", y.device());
+  c10::cuda::CUDAGuard guard(y.device());
+  check_rc(fdl_norm_rope_store(y.data_ptr(), rows > 1 ? y.stride(0) : y.size(1), positions.data_ptr<int64_t>(),
+                               inv_freq.data_ptr<float>(), as_int(inv_freq.numel(), "inv_freq"),
+                               q_weight ? q_weight->data_ptr() : nullptr, k_weight ? k_weight->data_ptr() : nullptr,
+                               static_cast<float>(eps), interleaved, static_cast<float>(rope_scale), q.data_ptr(),
+                               k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
+                               k_pages.stride(2), as_int(k_pages.size(0), "num_pages"),
+                               as_int(k_pages.size(1), "page_size"), slots.data_ptr<int64_t>(), rows,
+                               as_int(hq, "hq"), as_int(hkv, "hkv"), as_int(D, "D"), dtype_code(y), cur_stream()),
+           "norm_rope_store");
+}
+
+void paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+                       const Tensor& lens, double scale, const Tensor& out) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.stride(2) == 1,
+              "fdl.paged_decode_attn: q must be a CUDA [B, hq, D] tensor, contiguous in D");
+  TORCH_CHECK(out.is_cuda() && out.device() == q.device() && out.dtype() == q.dtype() && out.sizes() == q.sizes() &&
+                  out.stride(2) == 1,
+              "fdl.paged_decode_attn: out must match q, contiguous in D");
+  check_pages(k_pages, v_pages, q, "paged_decode_attn");
+  const int64_t B = q.size(0), hq = q.size(1), D = q.size(2), hkv = k_pages.size(2), page = k_pages.size(1);
+  TORCH_CHECK(k_pages.size(3) == D && hkv >= 1 && hq % hkv == 0, "fdl.paged_decode_attn: q ", q.sizes(),
+              " and pages ", k_pages.sizes(), " do not fit together");
+  check_table(block_table, q, B);
+  check_i32(lens, q, B, "lens");
+  c10::cuda::CUDAGuard guard(q.device());
+  const int64_t ws_bytes = fdl_paged_attn_workspace_bytes(as_int(B, "the batch"), as_int(hq, "hq"),
+                                                          as_int(hkv, "hkv"), as_int(D, "D"),
+                                                          block_table.size(1) * page);
+  Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+  check_rc(fdl_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
+                          k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), as_int(k_pages.size(0), "num_pages"),
+                          as_int(page, "page_size"), block_table.data_ptr<int32_t>(), table_stride(block_table),
+                          as_int(block_table.size(1), "max_pages"), lens.data_ptr<int32_t>(), static_cast<int>(B),
+                          static_cast<int>(hq), static_cast<int>(hkv), static_cast<int>(D), dtype_code(q),
+                          static_cast<float>(scale), out.data_ptr(), out.stride(0), out.stride(1),
+                          ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, cur_stream()),
+           "paged_decode_attn");
+}
+
+void token_logprobs(const Tensor& logits, const Tensor& targets, const Tensor& logprob, const Tensor& entropy,
+                    const std::optional<Tensor>& top_logprob, const std::optional<Tensor>& top_token) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
+              "fdl.token_logprobs: logits must be a CUDA [rows, vocab] tensor with unit inner stride");
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  check_i64(targets, logits, rows, "targets");
+  TORCH_CHECK(top_logprob.has_value() == top_token.has_value(),
+              "fdl.token_logprobs: top_logprob and top_token go together");
+  auto f32 = [&](const Tensor& t, int64_t n, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.device() == logits.device() && t.scalar_type() == at::kFloat && t.is_contiguous() &&
+                    t.numel() == n,
+                "fdl.token_logprobs: ", name, " must be a contiguous fp32 tensor of ", n, " entries on ",
+                logits.device());
+  };
+  f32(logprob, rows, "logprob");
+  f32(entropy, rows, "entropy");
+  int64_t top = 0;
+  if (top_logprob) {
+    TORCH_CHECK(top_logprob->dim() == 2, "fdl.token_logprobs: top_logprob must be [rows, top]");
+    top = top_logprob->size(1);
+    f32(*top_logprob, rows * top, "top_logprob");
+    check_i64(*top_token, logits, rows * top, "top_token");
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  check_rc(fdl_token_logprobs(logits.data_ptr(), rows > 1 ? logits.stride(0) : V, as_int(rows, "rows"),
+                              as_int(V, "the vocabulary"), dtype_code(logits), targets.data_ptr<int64_t>(),
+                              logprob.data_ptr<float>(), entropy.data_ptr<float>(), as_int(top, "top"),
+                              top_logprob ? top_logprob->data_ptr<float>() : nullptr,
+                              top_token ? top_token->data_ptr<int64_t>() : nullptr, cur_stream()),
+           "token_logprobs");
+}
+
 // Functional form with the signature of the flash_kvcache custom op of
 // utils/attention_backends.py:83-86; workspace comes from torch's caching
 // allocator (graph-capture safe).
@@ -673,6 +858,17 @@ TORCH_LIBRARY(fdl, m) {
         "Tensor(c!) v_dst, Tensor? start, Tensor? dst_pos, int seq_dim) -> ()");
   m.def("swiglu(Tensor gu, Tensor(a!) out) -> ()");
   m.def("softmax_argmax(Tensor logits, Tensor(a!) token, Tensor(b!)? prob) -> ()");
+  m.def("page_slots(Tensor(a!) lens, Tensor n_new, Tensor(b!) block_table, Tensor free_pages, Tensor(c!) free_count, "
+        "int page_size, Tensor(d!) slots, Tensor(e!) positions, Tensor(f!) cu_seqlens, Tensor(g!)? new_lens, "
+        "Tensor(h!)? new_count) -> ()");
+  m.def("page_release(Tensor done, Tensor(a!) lens, Tensor(b!) block_table, Tensor(c!) free_pages, "
+        "Tensor(d!) free_count, int page_size) -> ()");
+  m.def("norm_rope_store(Tensor y, Tensor positions, Tensor inv_freq, Tensor? q_weight, Tensor? k_weight, float eps, "
+        "bool interleaved, float rope_scale, Tensor(a!) q, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor slots) -> ()");
+  m.def("paged_decode_attn(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor lens, float scale, "
+        "Tensor(a!) out) -> ()");
+  m.def("token_logprobs(Tensor logits, Tensor targets, Tensor(a!) logprob, Tensor(b!) entropy, "
+        "Tensor(c!)? top_logprob, Tensor(d!)? top_token) -> ()");
   m.def("add_rmsnorm(Tensor x, Tensor res, Tensor? weight, float eps, Tensor(a!)? sum_out, Tensor(b!) normed) -> ()");
 }
 
@@ -694,6 +890,11 @@ TORCH_LIBRARY_IMPL(fdl, CUDA, m) {
   m.impl("swiglu", &swiglu);
   m.impl("softmax_argmax", &softmax_argmax);
   m.impl("add_rmsnorm", &add_rmsnorm);
+  m.impl("page_slots", &page_slots);
+  m.impl("page_release", &page_release);
+  m.impl("norm_rope_store", &norm_rope_store);
+  m.impl("paged_decode_attn", &paged_decode_attn);
+  m.impl("token_logprobs", &token_logprobs);
 }
 
 TORCH_LIBRARY_IMPL(fdl, Meta, m) {
@@ -725,6 +926,17 @@ TORCH_LIBRARY_IMPL(fdl, Meta, m) {
                            const Tensor&, const std::optional<Tensor>&, const std::optional<Tensor>&, int64_t) {});
   m.impl("swiglu", [](const Tensor&, const Tensor&) {});
   m.impl("softmax_argmax", [](const Tensor&, const Tensor&, const std::optional<Tensor>&) {});
+  m.impl("page_slots", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t,
+                          const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
+                          const std::optional<Tensor>&) {});
+  m.impl("page_release", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t) {});
+  m.impl("norm_rope_store",
+         [](const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, const std::optional<Tensor>&,
+            double, bool, double, const Tensor&, const Tensor&, const Tensor&, const Tensor&) {});
+  m.impl("paged_decode_attn", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, double,
+                                 const Tensor&) {});
+  m.impl("token_logprobs", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
+                              const std::optional<Tensor>&) {});
   m.impl("add_rmsnorm", [](const Tensor&, const Tensor&, const std::optional<Tensor>&, double,
                            const std::optional<Tensor>&, const Tensor&) {});
 }

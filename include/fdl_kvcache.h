@@ -439,6 +439,110 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
                        fdl_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Paged KV cache: a pool of pages shared by all sequences.  Pages are
+ * [num_pages, page_size, Hkv, D] (element strides kv_sp, kv_ss, kv_sh; the
+ * layer's K and V share them), table int32 [B, max_pages] (row stride
+ * table_sb) names the pages of a sequence, a slot is page * page_size +
+ * offset.  No counterpart in the reference except the page table it hands to
+ * FlashInfer's paged wrapper (utils/attention_backends.py:624-682).
+ *
+ * fdl_page_slots: table entries and slot map of n_new[b] more tokens per
+ * sequence, packed sequence after sequence into n_rows rows:
+ *   cu[b] = sum_{i<b} n_new[i] (cu has B + 1 entries)
+ *   positions[t] = lens[b] + t - cu[b],  slots[t] = its slot
+ * A sequence's new pages come off the end of free_pages[0 .. count[0]) (a
+ * stack; n_free is its capacity), in the order of the sequences, and are
+ * written into its table row behind the ceil(lens[b] / page_size) it has.
+ * new_lens[b] = lens[b] + n_new[b], new_count[0] = the pages left; both may be
+ * the inputs themselves (in place).  count is int32[2]: count[1] is scratch,
+ * 0 before and after a call, so calls on one count must not overlap.  A
+ * request that cannot be served (a negative length, no room in its table row,
+ * pages or rows that run out) is refused whole: slots -1, length unchanged, no
+ * page taken, FDL_DEV_LENGTH (info = b); sequences behind it that need pages
+ * are refused with it when the pool is what ran out.  Rows behind the last
+ * token get slot -1 and position 0.  batch <= 4096.
+ *
+ * fdl_page_release: for every b with done[b] (bytes, 0 or 1) the pages of the
+ * sequence go back onto the stack, its table entries become -1, its length 0.
+ * If the stack has no room for all of them, nothing changes and
+ * FDL_DEV_INDEX is reported.  The same count must not be used by another call
+ * at the same time.
+ *
+ * fdl_norm_rope_store: per row r of y [rows, (hq + 2 hkv) * D] (q, k and v
+ * heads; row stride y_rs): an RMS norm of every query head (weight q_weight
+ * [D], or none) and key head (k_weight), then the rotary positions over the
+ * first 2 * n_freq elements of the head -- pairs (j, j + n_freq), or (2j, 2j
+ * + 1) when interleaved -- by angle pos[r] * inv_freq[j], cos and sin scaled
+ * by rope_scale; q to q [rows, hq, D], k and v to their slot (slots int64
+ * [rows]; -1 stores nothing, any other slot outside the pool stores nothing
+ * and is reported).  Two rows may not name one slot.  All arithmetic is fp32
+ * (the angle fp64), rounded once.  bf16 or f16; D % 16 == 0, D <= 256, n_freq
+ * % 8 == 0, 2 * n_freq <= D.  Unlike fdl_rope_qkv_kv, which repeats the
+ * reference's bf16 roundings.
+ *
+ * fdl_paged_attn: attention of one query token per sequence,
+ *   out[b, h] = softmax_j(scale * q[b, h] . K[b, j, h / (hq / hkv)]) V[b, j, ..]
+ * over keys j < lens[b] (clamped to the table's width, FDL_DEV_LENGTH).  q and
+ * out [B, hq, D] with strides; bf16 or f16, D 64, 128 or 256.  A sequence
+ * without keys gives zeros.  A page outside [0, num_pages) hides its keys and
+ * is reported.  Softmax in fp32.  workspace: at least
+ * fdl_paged_attn_workspace_bytes() bytes, 16-byte aligned, not shared with a
+ * call that may run at the same time; its contents need not be kept.
+ * ---------------------------------------------------------------------- */
+int fdl_page_slots(const int32_t* lens, const int32_t* n_new, int batch,
+                   int32_t* table, int64_t table_sb, int max_pages,
+                   const int32_t* free_pages, int n_free, int32_t* count,
+                   int page_size, int64_t* slots, int64_t* positions,
+                   int64_t n_rows, int32_t* cu, int32_t* new_lens,
+                   int32_t* new_count, fdl_stream_t stream);
+int fdl_page_release(const uint8_t* done, int32_t* lens, int batch,
+                     int32_t* table, int64_t table_sb, int max_pages,
+                     int32_t* free_pages, int n_free, int32_t* count,
+                     int page_size, fdl_stream_t stream);
+int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos,
+                        const float* inv_freq, int n_freq,
+                        const void* q_weight, const void* k_weight, float eps,
+                        int interleaved, float rope_scale,
+                        void* q, void* k_pages, void* v_pages,
+                        int64_t kv_sp, int64_t kv_ss, int64_t kv_sh,
+                        int num_pages, int page_size, const int64_t* slots,
+                        int64_t rows, int hq, int hkv, int head_dim, int dtype,
+                        fdl_stream_t stream);
+int64_t fdl_paged_attn_workspace_bytes(int batch, int hq, int hkv, int head_dim,
+                                       int64_t max_len);
+int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh,
+                   const void* k_pages, const void* v_pages,
+                   int64_t kv_sp, int64_t kv_ss, int64_t kv_sh,
+                   int num_pages, int page_size,
+                   const int32_t* table, int64_t table_sb, int max_pages,
+                   const int32_t* lens, int batch, int hq, int hkv,
+                   int head_dim, int dtype, float scale,
+                   void* out, int64_t o_sb, int64_t o_sh,
+                   void* workspace, int64_t workspace_bytes,
+                   fdl_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Scores of given tokens over the vocabulary: for every row of logits [rows,
+ * vocab] (bf16, f16 or f32, row stride in elements, any alignment),
+ *   lse = ln sum_v exp(l_v),  logprob[r] = l_target - lse,
+ *   entropy[r] = -sum_v p_v ln p_v,  p_v = exp(l_v - lse),
+ *   top_token[r, :top], top_logprob[r, :top] = the top tokens of largest
+ *   logit, descending, the lower index first among equals, and l - lse.
+ * targets int64 [rows]: below 0 means no target (logprob 0); past the
+ * vocabulary gives NaN, reported as FDL_DEV_INDEX.  Logits of -inf count as
+ * probability 0.  A row with a NaN or +inf, or with nothing above -inf, is no
+ * distribution: NaN outputs, tokens -1, FDL_DEV_INDEX (info = row).  top <=
+ * 32 and top <= vocab; the top outputs may be NULL when top is 0.  Sums in
+ * fp32.  Stands next to fdl_softmax_argmax: the log-likelihoods that the
+ * reference's evaluation takes from whole log_softmax tensors.
+ * ---------------------------------------------------------------------- */
+int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows,
+                       int vocab, int dtype, const int64_t* targets,
+                       float* logprob, float* entropy, int top,
+                       float* top_logprob, int64_t* top_token,
+                       fdl_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Status.  Copies the calling device's first recorded device-side error
  * code into *code and the offending value into *info (either may be NULL),
  * then clears both.  Synchronises the device.  Returns 0 or -(cudaError_t).
