@@ -3,6 +3,7 @@
 // per-device status word declared in common.cuh.
 #include <cudaTypedefs.h>
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 #include <mutex>
 #include <type_traits>
@@ -52,6 +53,38 @@ bool make_map_4d(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uin
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+// Raises a kernel's shared-memory limit once per device.
+template <auto Kernel>
+bool smem_configured(int bytes) {
+  static std::atomic<uint64_t> done{0};  // one bit a device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
+// Paged attention: query heads a unit, grid, and whether units are shared
+// between CTAs (see paged_attn.cuh).
+struct PagedPlan {
+  int nh, grid;
+  bool joined;
+};
+constexpr int kPagedDirectKeys = 256;
+PagedPlan paged_plan(int batch, int hq, int hkv, int head_dim, int64_t cap) {
+  const int G = hq / hkv;
+  PagedPlan p{};
+  p.nh = G > 8 && head_dim < 256 ? 2 : 1;
+  const int64_t units = static_cast<int64_t>(batch) * hkv * ((G + 8 * p.nh - 1) / (8 * p.nh));
+  p.joined = cap > kPagedDirectKeys;
+  const int per_sm = head_dim == 64 && p.nh == 1 ? 3 : head_dim <= 128 ? 2 : 1;  // by shared memory
+  const int64_t tiles = units * ((cap + kPagedTile - 1) / kPagedTile);
+  p.grid = static_cast<int>(p.joined ? std::min<int64_t>(tiles, static_cast<int64_t>(num_sms()) * per_sm) : units);
+  return p;
 }
 
 bool attn_smem_configured() {
@@ -800,8 +833,10 @@ int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos, const f
 }
 
 int64_t fdl_paged_attn_workspace_bytes(int batch, int hq, int hkv, int head_dim, int64_t max_len) {
-  (void)batch; (void)hq; (void)hkv; (void)head_dim; (void)max_len;
-  return 0;
+  if (batch < 1 || hq < 1 || hkv < 1 || hq % hkv || max_len < 0) return 0;
+  const PagedPlan p = paged_plan(batch, hq, hkv, head_dim, max_len);
+  if (!p.joined) return 0;
+  return static_cast<int64_t>(p.grid) * (2 * 8 * p.nh * (static_cast<int64_t>(head_dim) * 4 + 8) + 16);
 }
 
 int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages, int64_t kv_sp,
@@ -810,8 +845,8 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
                    void* out, int64_t o_sb, int64_t o_sh, void* workspace, int64_t workspace_bytes,
                    fdl_stream_t stream) {
   if (dtype != FDL_BF16 && dtype != FDL_F16) return FDL_E_DTYPE;
-  if (batch < 0 || batch > 65535 || hq < 1 || hkv < 1 || hq % hkv || num_pages < 0 || page_size < 1 || max_pages < 0 ||
-      table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+  if (batch < 0 || batch > 65535 || hq < 1 || hq > 4096 || hkv < 1 || hq % hkv || num_pages < 0 || page_size < 1 ||
+      max_pages < 0 || table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX - kPagedTile)
     return FDL_E_SHAPE;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FDL_E_UNSUPPORTED;
   if (batch == 0) return FDL_OK;
@@ -820,21 +855,53 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
     if (!aligned16(p)) return FDL_E_ALIGN;
   for (int64_t st : {q_sb, q_sh, kv_sp, kv_ss, kv_sh, o_sb, o_sh})
     if ((st * 2) % 16) return FDL_E_ALIGN;
-  (void)workspace; (void)workspace_bytes;
+  const int cap = max_pages * page_size;
+  const PagedPlan plan = paged_plan(batch, hq, hkv, head_dim, cap);
+  const int H = 8 * plan.nh, G = hq / hkv, HG = (G + H - 1) / H;
   PagedAttnArgs a{q, q_sb, q_sh, static_cast<const char*>(k_pages), static_cast<const char*>(v_pages), kv_sp * 2,
-                  kv_ss * 2, kv_sh * 2, table, table_sb, lens, out, o_sb, o_sh, batch, hq, hkv, num_pages, max_pages,
-                  {}, scale * 1.4426950408889634f};
+                  kv_ss * 2, kv_sh * 2, table, table_sb, lens, out, o_sb, o_sh, batch, hq, hkv, num_pages, G, HG,
+                  hkv * HG, cap, {}, scale * 1.4426950408889634f, nullptr, nullptr, nullptr};
   a.page.init(static_cast<uint32_t>(page_size));
-  const dim3 grid(hq, batch);
+  if (plan.joined) {
+    if (!workspace || workspace_bytes < fdl_paged_attn_workspace_bytes(batch, hq, hkv, head_dim, cap))
+      return FDL_E_WORKSPACE;
+    if (!aligned16(workspace)) return FDL_E_ALIGN;
+    a.part_o = static_cast<float*>(workspace);
+    a.desc = reinterpret_cast<int4*>(a.part_o + static_cast<int64_t>(plan.grid) * 2 * H * head_dim);
+    a.part_ml = reinterpret_cast<float2*>(a.desc + plan.grid);
+  }
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) {
-    kernel<<<grid, kPagedThreads, 0, s>>>(a);
-    return launch_status();
+  auto go = [&](auto t, auto d, auto nh) -> int {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value, NH = decltype(nh)::value;
+    constexpr int smem = PagedCfg<D, NH>::kSmem;
+    if (!smem_configured<paged_attn_kernel<T, D, NH>>(smem)) return FDL_E_NODEVICE;
+    paged_attn_kernel<T, D, NH><<<plan.grid, kPagedThreads, smem, s>>>(a);
+    int rc = launch_status();
+    if (rc != FDL_OK || !plan.joined) return rc;
+    // The joining kernel may start while the first one runs (it waits for its
+    // end before it reads), which hides its launch.
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(plan.grid, std::min(G, H));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, NH>, a, plan.grid);
+    return e == cudaSuccess ? FDL_OK : -static_cast<int>(e);
+  };
+  auto by_nh = [&](auto t, auto d) {
+    if constexpr ((decltype(d)::value) < 256)
+      if (plan.nh == 2) return go(t, d, std::integral_constant<int, 2>{});
+    return go(t, d, std::integral_constant<int, 1>{});
   };
   auto by_d = [&](auto t) {
-    using T = decltype(t);
-    return head_dim == 64 ? go(paged_attn_kernel<T, 64>)
-                          : head_dim == 128 ? go(paged_attn_kernel<T, 128>) : go(paged_attn_kernel<T, 256>);
+    return head_dim == 64    ? by_nh(t, std::integral_constant<int, 64>{})
+           : head_dim == 128 ? by_nh(t, std::integral_constant<int, 128>{})
+                             : by_nh(t, std::integral_constant<int, 256>{});
   };
   return dtype == FDL_BF16 ? by_d(__nv_bfloat16{}) : by_d(__half{});
 }

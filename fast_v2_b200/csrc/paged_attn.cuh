@@ -5,10 +5,32 @@
 // A sequence without a visible key gives zeros.  A page outside the pool
 // hides its keys and is reported.
 //
-// One CTA per (sequence, query head): every warp walks its own keys with a
-// running maximum and sum, lanes share the head's elements, and the warps'
-// states are joined at the end.
+// Bound by HBM: every K and V row is read once for all query heads of its KV
+// head (2 * 2 * D bytes for 4 * D * G operations: at G = 7, 7 operations a
+// byte).  What has to be won is bytes in flight and an even share of them for
+// every SM, whatever the lengths.
+//
+// Unit = (sequence, KV head, group of 8 * NH query heads); its keys come in
+// tiles of 64.  The tiles of all units form one line, and each CTA of a grid
+// that fits the GPU takes an equal piece of it (found with one scan of the
+// lengths, on the device: lengths may change under a captured graph).  A unit
+// that lies in one piece is finished by its CTA; the pieces of the others go
+// to the workspace -- at most two a CTA, so the workspace does not grow with
+// the batch -- and a second kernel joins them in order.  Where the longest
+// possible sequence is short, a CTA takes a whole unit and there is nothing
+// to join.
+//
+// Within a CTA every warp takes 16 keys of a tile and runs on its own: its
+// rows arrive by cp.async in a ring of its own, no barrier between warps
+// until a unit ends.  Scores are formed transposed, S^T = K Q^T (m16n8k16:
+// 16 keys x 8 heads), and so is the output, O^T = V^T P^T: 8 query heads fill
+// the short side of the instruction, where Q on the long side would leave
+// half of it empty.  The matrix instructions are the warp-level ones: at 7
+// operations a byte they are far from busy, and an M = 128 instruction of the
+// tcgen05 kind would be 15/16 padding.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "norm_rope.cuh"
 
@@ -25,73 +47,482 @@ struct PagedAttnArgs {
   const int32_t* lens;
   void* out;
   int64_t o_sb, o_sh;
-  int B, hq, hkv, num_pages, max_pages;
+  int B, hq, hkv, num_pages;
+  int G, HG, NU;            // query heads a KV head, groups of them, units a sequence
+  int cap;                  // keys the table can name
   FastDiv page;
   float scale_log2;
+  // joining (null: every CTA takes one whole unit)
+  float* part_o;            // [2 grid, 8 NH, D] sums relative to the piece's reference
+  float2* part_ml;          // [2 grid, 8 NH] (reference, sum of p)
+  int4* desc;               // [grid] (sequence, unit of it) whose first piece ends the CTA's part of the line, or -1;
+                            // state of the CTA's first piece: 0 starts a unit, 1 middle of one, 2 end of one
 };
 
-constexpr int kPagedThreads = 128;
+constexpr int kPagedWarps = 4;
+constexpr int kPagedThreads = kPagedWarps * 32;
+constexpr int kPagedWarpKeys = 16;
+constexpr int kPagedTile = kPagedWarps * kPagedWarpKeys;
+// A score may pass the running reference by 2^8 before the sums are scaled
+// down to a new one (p <= 256 in either 16-bit type).
+constexpr float kPagedSlack = 8.f;
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
-  constexpr int E = D / 32;  // elements per lane
-  __shared__ float s_o[kPagedThreads / 32][D];
-  __shared__ float s_m[kPagedThreads / 32], s_l[kPagedThreads / 32];
-  const int b = blockIdx.y, h = blockIdx.x, kh = h / (a.hq / a.hkv);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int len = a.lens[b];
-  const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page.d;
-  if (len < 0 || len > cap) {
-    if (threadIdx.x == 0) report(FDL_DEV_LENGTH, b);
-    len = len < 0 ? 0 : static_cast<int>(cap);
-  }
-  const T* q = static_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + lane * E;
-  float qf[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qf[e] = static_cast<float>(q[e]) * a.scale_log2;
-    o[e] = 0.f;
-  }
-  for (int j = warp; j < len; j += kPagedThreads / 32) {
-    uint32_t i, r;
-    a.page.divmod(j, i, r);
-    const int page = a.table[b * a.table_sb + i];
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) report(FDL_DEV_INDEX, page);
-      continue;
+template <int D, int NH>
+struct PagedCfg {
+  static constexpr int kStages = D == 64 ? 4 : D == 128 ? (NH == 1 ? 3 : 2) : 2;
+  static constexpr int kStage = 2 * kPagedWarpKeys * D * 2;  // bytes: K rows, V rows
+  static constexpr int kRing = kPagedWarps * kStages * kStage;
+  static constexpr int kMergeRow = D + 4;  // floats: the four heads of a lane group land in different banks
+  static constexpr int kMerge = kPagedWarps * 8 * NH * kMergeRow * 4;
+  static constexpr int kSmem = kRing + kMerge;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const char* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) { return min(max(a.lens[b], 0), a.cap); }
+
+// A place on the line of tiles.
+struct PagedPos {
+  int b, n;      // sequence, unit of the sequence
+  int t, nt;     // tile of the unit, tiles of a unit of b
+  int len;
+  __device__ __forceinline__ void next(const PagedAttnArgs& a) {
+    if (++t < nt) return;
+    t = 0;
+    if (++n < a.NU) return;
+    n = 0;
+    for (++b; b < a.B; ++b) {
+      len = paged_len(a, b);
+      nt = (len + kPagedTile - 1) / kPagedTile;
+      if (nt > 0) return;
     }
-    const int64_t at = page * a.sp + r * a.ss + kh * a.sh;
-    const T* k = reinterpret_cast<const T*>(a.k + at) + lane * E;
-    const T* v = reinterpret_cast<const T*>(a.v + at) + lane * E;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(qf[e], static_cast<float>(k[e]), s);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    const float mn = fmaxf(m, s);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float p = exp2f(s - ref), c = exp2f(m - ref);
-    l = l * c + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(p, static_cast<float>(v[e]), o[e] * c);
-    m = mn;
   }
+};
+
+template <typename T, int D, int NH>
+__global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+  using Cfg = PagedCfg<D, NH>;
+  constexpr int kStages = Cfg::kStages, kChunks = D / 8, kRowB = D * 2, H = 8 * NH;
+  constexpr int kLoads = kPagedWarpKeys * kChunks / 32;  // 16-byte pieces of K (and of V) a lane and tile
+  extern __shared__ __align__(128) char smem[];
+  __shared__ int s_mask[kPagedWarps][kStages];
+  __shared__ float2 s_ml[kPagedWarps][H];
+  __shared__ int s_pos[4];
+  __shared__ long long s_scan[kPagedWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c4 = lane & 3;
+  float* s_merge = reinterpret_cast<float*>(smem + Cfg::kRing);
+  const uint32_t ring = smem_addr(smem) + warp * kStages * Cfg::kStage;
+  T* const out = static_cast<T*>(a.out);
+
+  // ---- this CTA's piece of the line
+  PagedPos p{};
+  int left;  // tiles
+  bool joined = a.part_o != nullptr;
+  if (joined) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int per = (a.B + kPagedThreads - 1) / kPagedThreads;
+    const int b0 = threadIdx.x * per, b1 = min(a.B, b0 + per);
+    long long sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int raw = a.lens[b];
+      if (blockIdx.x == 0 && (raw < 0 || raw > a.cap)) report(FDL_DEV_LENGTH, b);
+      sum += (min(max(raw, 0), a.cap) + kPagedTile - 1) / kPagedTile;
+    }
+    long long incl = sum;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += o;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) {
+      if (w < warp) incl += s_scan[w];
+      total += s_scan[w];
+    }
+    total *= a.NU;
+    // no CTA before the last busy one is without tiles, so pieces of a unit
+    // lie on consecutive CTAs
+    const long long busy = min(static_cast<long long>(gridDim.x), total);
+    long long first = 0;
+    left = 0;
+    if (blockIdx.x < busy) {
+      first = total * blockIdx.x / busy;
+      left = static_cast<int>(total * (blockIdx.x + 1) / busy - first);
+    }
+    long long at = (incl - sum) * a.NU;
+    if (left > 0 && first >= at && first < incl * a.NU) {
+      for (int b = b0; b < b1; ++b) {
+        const int len = paged_len(a, b), nt = (len + kPagedTile - 1) / kPagedTile;
+        const long long mine = static_cast<long long>(nt) * a.NU;
+        if (first < at + mine) {
+          const int local = static_cast<int>(first - at);
+          s_pos[0] = b;
+          s_pos[1] = local / nt;
+          s_pos[2] = local % nt;
+          s_pos[3] = len;
+          break;
+        }
+        at += mine;
+      }
+    }
+    // Sequences without keys: shared out over the grid.
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (paged_len(a, b) == 0)
+        for (int i = threadIdx.x; i < a.hq * kChunks; i += kPagedThreads)
+          *reinterpret_cast<uint4*>(out + b * a.o_sb + (i / kChunks) * a.o_sh + (i % kChunks) * 8) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    if (left == 0) {
+      if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
+    p.b = s_pos[0];
+    p.n = s_pos[1];
+    p.t = s_pos[2];
+    p.len = s_pos[3];
+  } else {
+    p.b = blockIdx.x / a.NU;
+    p.n = blockIdx.x % a.NU;
+    const int raw = a.lens[p.b];
+    if (p.n == 0 && threadIdx.x == 0 && (raw < 0 || raw > a.cap)) report(FDL_DEV_LENGTH, p.b);
+    p.len = paged_len(a, p.b);
+    left = (p.len + kPagedTile - 1) / kPagedTile;
+    if (left == 0) {
+      const int h0 = (p.n / a.HG) * a.G + (p.n % a.HG) * H, hn = min(H, a.G - (p.n % a.HG) * H);
+      for (int i = threadIdx.x; i < hn * kChunks; i += kPagedThreads)
+        *reinterpret_cast<uint4*>(out + p.b * a.o_sb + (h0 + i / kChunks) * a.o_sh + (i % kChunks) * 8) =
+            make_uint4(0, 0, 0, 0);
+      return;
+    }
   }
-  __syncthreads();
-  float M = -INFINITY, Lsum = 0.f;
-  for (int w = 0; w < kPagedThreads / 32; ++w) M = fmaxf(M, s_m[w]);
+  p.nt = (p.len + kPagedTile - 1) / kPagedTile;
+  // 0: the first piece starts its unit
+  int state = p.t == 0 ? 0 : (p.t + left >= p.nt ? 2 : 1);
+  const int first_state = state;
+
+  // ---- loads: the warp's 16 rows of tile `w`, with the pages looked up one tile ahead
+  PagedPos w = p;  // next tile to load
+  int w_left = left;
+  const bool whole = a.page.d % kPagedWarpKeys == 0;  // the 16 keys lie in one page
+  int page = 0;
+  auto look_up = [&]() {  // the page of this lane's key of tile w
+    if (w_left > 0) {
+      const int key = w.t * kPagedTile + warp * kPagedWarpKeys + (whole ? 0 : lane & 15);
+      page = key < w.len ? a.table[w.b * a.table_sb + a.page.div(key)] : 0;
+    }
+  };
+  int fill = 0;
+  auto load = [&]() {
+    if (w_left > 0) {
+      const int key0 = w.t * kPagedTile + warp * kPagedWarpKeys;
+      if (key0 < w.len) {
+        const int key = key0 + (lane & 15);
+        bool ok = key < w.len;
+        if (ok && (page < 0 || page >= a.num_pages)) {
+          if (lane < 16) report(FDL_DEV_INDEX, page);
+          ok = false;
+        }
+        const unsigned mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+        if (lane == 0) s_mask[warp][fill] = mask;
+        const int pk = whole ? key0 : key;
+        const int64_t off = static_cast<int64_t>(page) * a.sp +
+                            static_cast<int64_t>(static_cast<uint32_t>(pk) - a.page.div(pk) * a.page.d) * a.ss +
+                            static_cast<int64_t>(w.n / a.HG) * a.sh;
+        const uint32_t dst = ring + fill * Cfg::kStage;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int piece = i * 32 + lane;
+          const int r = piece / kChunks, ch = piece % kChunks;
+          const int64_t row = whole ? off + r * a.ss : __shfl_sync(0xffffffffu, off, r);
+          const bool get = (mask >> r) & 1;
+          const int64_t at = get ? row + ch * 16 : 0;
+          const uint32_t to = dst + r * kRowB + ((ch ^ (r & 7)) * 16);
+          cp_async16(to, a.k + at, get ? 16 : 0);
+          cp_async16(to + kPagedWarpKeys * kRowB, a.v + at, get ? 16 : 0);
+        }
+      }
+      if (--w_left > 0) w.next(a);
+    }
+    cp_commit();
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+    look_up();
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load();
+
+  uint32_t qf[NH][D / 16][2];
+  float o[NH][D / 16][4];
+  float m[NH][2], l[NH][2];
+  int use = 0;
+  bool fresh = true;
+  while (left > 0) {
+    const int kh = p.n / a.HG, h0 = kh * a.G + (p.n % a.HG) * H, hn = min(H, a.G - (p.n % a.HG) * H);
+    if (fresh) {
+      fresh = false;
+      const T* q = static_cast<const T*>(a.q) + p.b * a.q_sb + h0 * a.q_sh;
+#pragma unroll
+      for (int x = 0; x < NH; ++x) {
+        const int hh = x * 8 + g;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            qf[x][kk][e] = hh < hn ? *reinterpret_cast<const uint32_t*>(q + hh * a.q_sh + kk * 16 + e * 8 + c4 * 2) : 0u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[x][kk][e] = 0.f;
+        }
+        m[x][0] = m[x][1] = -INFINITY;
+        l[x][0] = l[x][1] = 0.f;
+      }
+    }
+    __syncwarp();  // the slot that is loaded next has been read
+    load();
+    cp_wait<kStages - 1>();
+    __syncwarp();
+    if (p.t * kPagedTile + warp * kPagedWarpKeys < p.len) {
+      const uint32_t kb = ring + use * Cfg::kStage, vb = kb + kPagedWarpKeys * kRowB;
+      const unsigned mask = s_mask[warp][use];
+      float s[NH][2][4];
+#pragma unroll
+      for (int x = 0; x < NH; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[x][0][e] = s[x][1][e] = 0.f;
+      {
+        const int r = lane & 15;
+        const uint32_t row = kb + r * kRowB;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t f[4];
+          ldsm4(f, row + (((kk * 2 + (lane >> 4)) ^ (r & 7)) * 16));
+#pragma unroll
+          for (int x = 0; x < NH; ++x) mma16816<T>(s[x][kk & 1], f, qf[x][kk][0], qf[x][kk][1]);
+        }
+      }
+      uint32_t pf[NH][2];
+#pragma unroll
+      for (int x = 0; x < NH; ++x) {
+        float v[4];  // keys g, g, g + 8, g + 8 of heads 2 c4, 2 c4 + 1
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (s[x][0][e] + s[x][1][e]) * a.scale_log2;
+        if (mask != 0xffffu) {
+          if (!((mask >> g) & 1)) v[0] = v[1] = -INFINITY;
+          if (!((mask >> (g + 8)) & 1)) v[2] = v[3] = -INFINITY;
+        }
+        float t0 = fmaxf(v[0], v[2]), t1 = fmaxf(v[1], v[3]);
+        if (__any_sync(0xffffffffu, t0 > m[x][0] + kPagedSlack || t1 > m[x][1] + kPagedSlack)) {
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+          }
+          const float n0 = fmaxf(m[x][0], t0), n1 = fmaxf(m[x][1], t1);
+          const float f0 = n0 == -INFINITY ? 1.f : ex2(m[x][0] - n0), f1 = n1 == -INFINITY ? 1.f : ex2(m[x][1] - n1);
+          m[x][0] = n0;
+          m[x][1] = n1;
+          l[x][0] *= f0;
+          l[x][1] *= f1;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            o[x][kk][0] *= f0;
+            o[x][kk][1] *= f1;
+            o[x][kk][2] *= f0;
+            o[x][kk][3] *= f1;
+          }
+        }
+        const float r0 = m[x][0] == -INFINITY ? 0.f : m[x][0], r1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
+        // P is rounded to the type of V for the product, and the sum takes
+        // the rounded values, so that a weight's rounding cancels where one
+        // key dominates.
+        const uint32_t p0 = Pack2<T>::from(ex2(v[0] - r0), ex2(v[1] - r1));
+        const uint32_t p1 = Pack2<T>::from(ex2(v[2] - r0), ex2(v[3] - r1));
+        const float2 q0 = Pack2<T>::to(p0), q1 = Pack2<T>::to(p1);
+        l[x][0] += q0.x + q1.x;
+        l[x][1] += q0.y + q1.y;
+        pf[x][0] = movmatrix_t(p0);
+        pf[x][1] = movmatrix_t(p1);
+      }
+      {
+        const int r = (lane & 7) | ((lane >> 4) << 3);
+        const uint32_t row = vb + r * kRowB;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t f[4];
+          ldsm4_t(f, row + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
+#pragma unroll
+          for (int x = 0; x < NH; ++x) mma16816<T>(o[x][kk], f, pf[x][0], pf[x][1]);
+        }
+      }
+    }
+    use = use + 1 == kStages ? 0 : use + 1;
+    --left;
+    const bool ends = p.t + 1 == p.nt;
+    if (ends || left == 0) {
+      // ---- join the warps; finish the unit, or leave the piece in the workspace
+#pragma unroll
+      for (int x = 0; x < NH; ++x) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], off);
+        if (g == 0) {
+          s_ml[warp][x * 8 + c4 * 2] = make_float2(m[x][0], l[x][0]);
+          s_ml[warp][x * 8 + c4 * 2 + 1] = make_float2(m[x][1], l[x][1]);
+        }
+        float* mo = s_merge + (warp * H + x * 8 + c4 * 2) * Cfg::kMergeRow;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          mo[kk * 16 + g] = o[x][kk][0];
+          mo[Cfg::kMergeRow + kk * 16 + g] = o[x][kk][1];
+          mo[kk * 16 + g + 8] = o[x][kk][2];
+          mo[Cfg::kMergeRow + kk * 16 + g + 8] = o[x][kk][3];
+        }
+      }
+      __syncthreads();
+      const bool all = state == 0 && ends;
+      const int slot = blockIdx.x * 2 + (state == 0 ? 1 : 0);
+      for (int i = threadIdx.x; i < hn * kChunks; i += kPagedThreads) {
+        const int hh = i / kChunks, ch = i % kChunks;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int x = 0; x < kPagedWarps; ++x) M = fmaxf(M, s_ml[x][hh].x);
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int x = 0; x < kPagedWarps; ++x) {
+          const float2 ml = s_ml[x][hh];
+          const float f = ex2(ml.x - ref);
+          L = fmaf(ml.y, f, L);
+          const float4* src = reinterpret_cast<const float4*>(s_merge + (x * H + hh) * Cfg::kMergeRow + ch * 8);
+          const float4 u0 = src[0], u1 = src[1];
+          acc[0] = fmaf(u0.x, f, acc[0]);
+          acc[1] = fmaf(u0.y, f, acc[1]);
+          acc[2] = fmaf(u0.z, f, acc[2]);
+          acc[3] = fmaf(u0.w, f, acc[3]);
+          acc[4] = fmaf(u1.x, f, acc[4]);
+          acc[5] = fmaf(u1.y, f, acc[5]);
+          acc[6] = fmaf(u1.z, f, acc[6]);
+          acc[7] = fmaf(u1.w, f, acc[7]);
+        }
+        if (all) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] *= inv;
+          *reinterpret_cast<uint4*>(out + p.b * a.o_sb + (h0 + hh) * a.o_sh + ch * 8) = pack8<T>(acc);
+        } else {
+          float4* dst = reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(slot) * H + hh) * D + ch * 8);
+          dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+          if (ch == 0) a.part_ml[slot * H + hh] = make_float2(M, L);
+        }
+      }
+      if (joined && left == 0 && threadIdx.x == 0)
+        a.desc[blockIdx.x] = make_int4(state == 0 && !ends ? p.b : -1, p.n, first_state, 0);
+      __syncthreads();  // s_merge and s_ml are free again
+      fresh = true;
+      state = 0;
+    }
+    if (left > 0) p.next(a);
+  }
+  cp_wait<0>();
+}
+
+// Joins the pieces of the units that lie on more than one CTA: CTA (c, h)
+// takes query head h of the unit whose first piece ends CTA c's part of the
+// line; its other pieces are the first ones of the CTAs behind c, up to the
+// one that ends the unit.  Warps take pieces in turn and are joined in order.
+template <typename T, int D, int NH>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int grid) {
+  constexpr int H = 8 * NH, E = D / 32;
+  __shared__ float s_o[4][D];
+  __shared__ float s_l[4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x, hh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 d = a.desc[c];
+  if (d.x < 0) return;
+  const int g0 = (d.y % a.HG) * H;
+  if (hh >= min(H, a.G - g0)) return;
+  int last = c + 1;
+  while (last < grid - 1 && a.desc[last].z != 2) ++last;
+  // reference of all pieces
+  float M = -INFINITY;
+  for (int i = c + lane; i <= last; i += 32) M = fmaxf(M, a.part_ml[(i * 2 + (i == c)) * H + hh].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
   const float ref = M == -INFINITY ? 0.f : M;
-  for (int w = 0; w < kPagedThreads / 32; ++w) Lsum += s_l[w] * exp2f(s_m[w] - ref);
-  T* out = static_cast<T*>(a.out) + b * a.o_sb + h * a.o_sh;
-  for (int d = threadIdx.x; d < D; d += kPagedThreads) {
-    float x = 0.f;
-    for (int w = 0; w < kPagedThreads / 32; ++w) x += s_o[w][d] * exp2f(s_m[w] - ref);
-    out[d] = static_cast<T>(Lsum > 0.f || Lsum != Lsum ? x / Lsum : 0.f);
+  float acc[E], L = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int i = c + warp; i <= last; i += 4) {
+    const int slot = (i * 2 + (i == c)) * H + hh;
+    const float2 ml = a.part_ml[slot];
+    const float* src = a.part_o + static_cast<int64_t>(slot) * D + lane;
+    const float f = ex2(ml.x - ref);
+    L = fmaf(ml.y, f, L);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e * 32], f, acc[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_o[warp][e * 32 + lane] = acc[e];
+  if (lane == 0) s_l[warp] = L;
+  __syncthreads();
+  const float l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(a.out) + d.x * a.o_sb + ((d.y / a.HG) * a.G + g0 + hh) * a.o_sh;
+  for (int i = threadIdx.x; i < D / 2; i += 128) {
+    float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      x0 += s_o[w][2 * i];
+      x1 += s_o[w][2 * i + 1];
+    }
+    reinterpret_cast<uint32_t*>(out)[i] = Pack2<T>::from(x0 * inv, x1 * inv);
   }
 }
 
