@@ -82,6 +82,9 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cas
 __device__ __forceinline__ void cp_async16(uint32_t dst, const char* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const char* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
@@ -122,6 +125,15 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) { return min(max(a.lens[b], 0), a.cap); }
+
+// n / f.d for n < 2^31 (FastDiv::div with the 32-bit halves of the product
+// spelled out: two multiplies).
+__device__ __forceinline__ int paged_div(const FastDiv& f, int n) {
+  if (f.d == 1) return n;
+  const uint64_t lo = static_cast<uint64_t>(static_cast<uint32_t>(f.m)) * static_cast<uint32_t>(n);
+  const uint64_t hi = (f.m >> 32) * static_cast<uint32_t>(n) + (lo >> 32);
+  return static_cast<int>(hi >> 32);
+}
 
 // A place on the line of tiles.
 struct PagedPos {
@@ -246,44 +258,74 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
   const int first_state = state;
 
   // ---- loads: the warp's 16 rows of tile `w`, with the pages looked up one tile ahead
+  constexpr int kRows = 32 / kChunks;  // rows a warp-wide copy covers (D = 64: 4, 128: 2, 256: 1)
   PagedPos w = p;  // next tile to load
   int w_left = left;
   const bool whole = a.page.d % kPagedWarpKeys == 0;  // the 16 keys lie in one page
-  int page = 0;
+  const int64_t lane_src = static_cast<int64_t>(lane / kChunks) * a.ss + (lane % kChunks) * 16;
+  const int64_t step_src = a.ss * kRows;
+  const int64_t v_minus_k = a.v - a.k;
+  // Row r holds its 16-byte piece ch at ch ^ (r & 7): eight rows of one piece
+  // lie in different banks.  Offsets of this lane, by what they depend on.
+  uint32_t to_off[8 / kRows], k_off[4], v_off[4];
+#pragma unroll
+  for (int i = 0; i < 8 / kRows; ++i) {
+    const int r = i * kRows + lane / kChunks;
+    to_off[i] = r * kRowB + (((lane % kChunks) ^ (r & 7)) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rk = lane & 15, rv = (lane & 7) | ((lane >> 4) << 3);
+    k_off[i] = rk * kRowB + (((i * 2 + (lane >> 4)) ^ (rk & 7)) * 16);
+    v_off[i] = kPagedWarpKeys * kRowB + rv * kRowB + (((i * 2 + ((lane >> 3) & 1)) ^ (rv & 7)) * 16);
+  }
+  int page = 0, in_page = 0;
   auto look_up = [&]() {  // the page of this lane's key of tile w
     if (w_left > 0) {
       const int key = w.t * kPagedTile + warp * kPagedWarpKeys + (whole ? 0 : lane & 15);
-      page = key < w.len ? a.table[w.b * a.table_sb + a.page.div(key)] : 0;
+      if (key < w.len) {
+        const int i = paged_div(a.page, key);
+        in_page = key - i * static_cast<int>(a.page.d);
+        page = a.table[w.b * a.table_sb + i];
+      }
     }
   };
   int fill = 0;
   auto load = [&]() {
     if (w_left > 0) {
-      const int key0 = w.t * kPagedTile + warp * kPagedWarpKeys;
-      if (key0 < w.len) {
-        const int key = key0 + (lane & 15);
-        bool ok = key < w.len;
-        if (ok && (page < 0 || page >= a.num_pages)) {
-          if (lane < 16) report(FDL_DEV_INDEX, page);
-          ok = false;
-        }
-        const unsigned mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        if (lane == 0) s_mask[warp][fill] = mask;
-        const int pk = whole ? key0 : key;
-        const int64_t off = static_cast<int64_t>(page) * a.sp +
-                            static_cast<int64_t>(static_cast<uint32_t>(pk) - a.page.div(pk) * a.page.d) * a.ss +
+      const int n = w.len - w.t * kPagedTile - warp * kPagedWarpKeys;  // keys from the warp's first on
+      if (n > 0) {
+        const bool bad = static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_pages);
+        const int64_t off = static_cast<int64_t>(page) * a.sp + static_cast<int64_t>(in_page) * a.ss +
                             static_cast<int64_t>(w.n / a.HG) * a.sh;
         const uint32_t dst = ring + fill * Cfg::kStage;
+        if (whole && n >= kPagedWarpKeys && !bad) {
+          if (lane == 0) s_mask[warp][fill] = 0xffff;
+          const char* src = a.k + off + lane_src;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int piece = i * 32 + lane;
-          const int r = piece / kChunks, ch = piece % kChunks;
-          const int64_t row = whole ? off + r * a.ss : __shfl_sync(0xffffffffu, off, r);
-          const bool get = (mask >> r) & 1;
-          const int64_t at = get ? row + ch * 16 : 0;
-          const uint32_t to = dst + r * kRowB + ((ch ^ (r & 7)) * 16);
-          cp_async16(to, a.k + at, get ? 16 : 0);
-          cp_async16(to + kPagedWarpKeys * kRowB, a.v + at, get ? 16 : 0);
+          for (int i = 0; i < kLoads; ++i) {
+            const uint32_t to = dst + to_off[i % (8 / kRows)] + (i / (8 / kRows)) * 8 * kRowB;
+            cp_async16(to, src);
+            cp_async16(to + kPagedWarpKeys * kRowB, src + v_minus_k);
+            src += step_src;
+          }
+        } else {
+          // the last keys of a sequence, bad pages, pages that end inside
+          // the 16 keys: row by row, zeros in place of what is not there
+          const bool in = (lane & 15) < n;
+          if (in && bad && lane < 16) report(FDL_DEV_INDEX, page);
+          const unsigned mask = __ballot_sync(0xffffffffu, in && !bad) & 0xffffu;
+          if (lane == 0) s_mask[warp][fill] = mask;
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const int r = i * kRows + lane / kChunks;
+            const int64_t row = whole ? off + r * a.ss : __shfl_sync(0xffffffffu, off, r);
+            const bool get = (mask >> r) & 1;
+            const int64_t at = get ? row + (lane % kChunks) * 16 : 0;
+            const uint32_t to = dst + to_off[i % (8 / kRows)] + (i / (8 / kRows)) * 8 * kRowB;
+            cp_async16(to, a.k + at, get ? 16 : 0);
+            cp_async16(to + kPagedWarpKeys * kRowB, a.v + at, get ? 16 : 0);
+          }
         }
       }
       if (--w_left > 0) w.next(a);
@@ -326,23 +368,19 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
     cp_wait<kStages - 1>();
     __syncwarp();
     if (p.t * kPagedTile + warp * kPagedWarpKeys < p.len) {
-      const uint32_t kb = ring + use * Cfg::kStage, vb = kb + kPagedWarpKeys * kRowB;
+      const uint32_t slot = ring + use * Cfg::kStage;
       const unsigned mask = s_mask[warp][use];
       float s[NH][2][4];
 #pragma unroll
       for (int x = 0; x < NH; ++x)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[x][0][e] = s[x][1][e] = 0.f;
-      {
-        const int r = lane & 15;
-        const uint32_t row = kb + r * kRowB;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          uint32_t f[4];
-          ldsm4(f, row + (((kk * 2 + (lane >> 4)) ^ (r & 7)) * 16));
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t f[4];
+        ldsm4(f, slot + k_off[kk & 3] + (kk >> 2) * 128);
 #pragma unroll
-          for (int x = 0; x < NH; ++x) mma16816<T>(s[x][kk & 1], f, qf[x][kk][0], qf[x][kk][1]);
-        }
+        for (int x = 0; x < NH; ++x) mma16816<T>(s[x][kk & 1], f, qf[x][kk][0], qf[x][kk][1]);
       }
       uint32_t pf[NH][2];
 #pragma unroll
@@ -387,16 +425,12 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
         pf[x][0] = movmatrix_t(p0);
         pf[x][1] = movmatrix_t(p1);
       }
-      {
-        const int r = (lane & 7) | ((lane >> 4) << 3);
-        const uint32_t row = vb + r * kRowB;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          uint32_t f[4];
-          ldsm4_t(f, row + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t f[4];
+        ldsm4_t(f, slot + v_off[kk & 3] + (kk >> 2) * 128);
 #pragma unroll
-          for (int x = 0; x < NH; ++x) mma16816<T>(o[x][kk], f, pf[x][0], pf[x][1]);
-        }
+        for (int x = 0; x < NH; ++x) mma16816<T>(o[x][kk], f, pf[x][0], pf[x][1]);
       }
     }
     use = use + 1 == kStages ? 0 : use + 1;
@@ -425,7 +459,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
       }
       __syncthreads();
       const bool all = state == 0 && ends;
-      const int slot = blockIdx.x * 2 + (state == 0 ? 1 : 0);
+      const int piece = blockIdx.x * 2 + (state == 0 ? 1 : 0);
       for (int i = threadIdx.x; i < hn * kChunks; i += kPagedThreads) {
         const int hh = i / kChunks, ch = i % kChunks;
         float M = -INFINITY, L = 0.f;
@@ -455,10 +489,10 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
           for (int e = 0; e < 8; ++e) acc[e] *= inv;
           *reinterpret_cast<uint4*>(out + p.b * a.o_sb + (h0 + hh) * a.o_sh + ch * 8) = pack8<T>(acc);
         } else {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(slot) * H + hh) * D + ch * 8);
+          float4* dst = reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(piece) * H + hh) * D + ch * 8);
           dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
           dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-          if (ch == 0) a.part_ml[slot * H + hh] = make_float2(M, L);
+          if (ch == 0) a.part_ml[piece * H + hh] = make_float2(M, L);
         }
       }
       if (joined && left == 0 && threadIdx.x == 0)
@@ -480,47 +514,74 @@ template <typename T, int D, int NH>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int grid) {
   constexpr int H = 8 * NH, E = D / 32;
   __shared__ float s_o[4][D];
-  __shared__ float s_l[4];
+  __shared__ float2 s_ml[4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x, hh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4 d = a.desc[c];
   if (d.x < 0) return;
   const int g0 = (d.y % a.HG) * H;
   if (hh >= min(H, a.G - g0)) return;
-  int last = c + 1;
-  while (last < grid - 1 && a.desc[last].z != 2) ++last;
-  // reference of all pieces
-  float M = -INFINITY;
-  for (int i = c + lane; i <= last; i += 32) M = fmaxf(M, a.part_ml[(i * 2 + (i == c)) * H + hh].x);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  const float ref = M == -INFINITY ? 0.f : M;
-  float acc[E], L = 0.f;
+  // the piece that ends the unit: the first CTA behind c in that state
+  int last = c;
+  for (int i0 = c + 1; i0 < grid; i0 += 32) {
+    const unsigned end = __ballot_sync(0xffffffffu, i0 + lane < grid && a.desc[i0 + lane].z == 2);
+    last = end ? i0 + __ffs(end) - 1 : min(i0 + 31, grid - 1);
+    if (end) break;
+  }
+  // Each warp keeps a reference of its own, four pieces at a time.
+  float acc[E], L = 0.f, M = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int i = c + warp; i <= last; i += 4) {
-    const int slot = (i * 2 + (i == c)) * H + hh;
-    const float2 ml = a.part_ml[slot];
-    const float* src = a.part_o + static_cast<int64_t>(slot) * D + lane;
-    const float f = ex2(ml.x - ref);
-    L = fmaf(ml.y, f, L);
+  for (int i0 = c + warp; i0 <= last; i0 += 16) {
+    float2 ml[4];
+    float x[4][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e * 32], f, acc[e]);
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * 4;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      if (i <= last) {
+        const int slot = (i * 2 + (i == c)) * H + hh;
+        ml[u] = a.part_ml[slot];
+        const float* src = a.part_o + static_cast<int64_t>(slot) * D + lane;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = src[e * 32];
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+      }
+    }
+    const float n = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+    const float ref = n == -INFINITY ? 0.f : n;
+    const float f = ex2(M - ref);
+    M = n;
+    L *= f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float g = ex2(ml[u].x - ref);
+      L = fmaf(ml[u].y, g, L);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(x[u][e], g, acc[e]);
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) s_o[warp][e * 32 + lane] = acc[e];
-  if (lane == 0) s_l[warp] = L;
+  if (lane == 0) s_ml[warp] = make_float2(M, L);
   __syncthreads();
-  const float l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  const float2 m0 = s_ml[0], m1 = s_ml[1], m2 = s_ml[2], m3 = s_ml[3];
+  const float top = fmaxf(fmaxf(m0.x, m1.x), fmaxf(m2.x, m3.x));
+  const float ref = top == -INFINITY ? 0.f : top;
+  const float f[4] = {ex2(m0.x - ref), ex2(m1.x - ref), ex2(m2.x - ref), ex2(m3.x - ref)};
+  const float l = m0.y * f[0] + m1.y * f[1] + m2.y * f[2] + m3.y * f[3];
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* out = static_cast<T*>(a.out) + d.x * a.o_sb + ((d.y / a.HG) * a.G + g0 + hh) * a.o_sh;
   for (int i = threadIdx.x; i < D / 2; i += 128) {
     float x0 = 0.f, x1 = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      x0 += s_o[w][2 * i];
-      x1 += s_o[w][2 * i + 1];
+      x0 = fmaf(s_o[w][2 * i], f[w], x0);
+      x1 = fmaf(s_o[w][2 * i + 1], f[w], x1);
     }
     reinterpret_cast<uint32_t*>(out)[i] = Pack2<T>::from(x0 * inv, x1 * inv);
   }
