@@ -68,22 +68,41 @@ bool smem_configured(int bytes) {
   return true;
 }
 
-// Paged attention: query heads a unit, grid, and whether units are shared
-// between CTAs (see paged_attn.cuh).
+// Paged attention: query heads a unit, warps a CTA, and how the units are
+// shared out (see paged_attn.cuh).
 struct PagedPlan {
-  int nh, grid;
-  bool joined;
+  int nh, nw, grid;
+  int cluster;  // 0: line
 };
-constexpr int kPagedDirectKeys = 256;
 PagedPlan paged_plan(int batch, int hq, int hkv, int head_dim, int64_t cap) {
   const int G = hq / hkv;
   PagedPlan p{};
   p.nh = G > 8 && head_dim < 256 ? 2 : 1;
   const int64_t units = static_cast<int64_t>(batch) * hkv * ((G + 8 * p.nh - 1) / (8 * p.nh));
-  p.joined = cap > kPagedDirectKeys;
-  const int per_sm = head_dim == 64 && p.nh == 1 ? 3 : head_dim <= 128 ? 2 : 1;  // by shared memory
-  const int64_t tiles = units * ((cap + kPagedTile - 1) / kPagedTile);
-  p.grid = static_cast<int>(p.joined ? std::min<int64_t>(tiles, static_cast<int64_t>(num_sms()) * per_sm) : units);
+  // Clusters of up to 8 CTAs of 8 warps while they fit the GPU side by side;
+  // with more units, one CTA of 4 warps each.  A cluster's time follows its
+  // own sequence (0.7 us a tile and CTA), so a batch in which one sequence is
+  // long waits for it; the line costs a scan and a second kernel, but shares
+  // any batch out evenly.  Measured on B200, 28 query / 4 KV heads of 128, all
+  // sequences of one length, cluster against line: 320 keys B=1 5.5 / 6.3 us,
+  // B=30 6.0 / 10.4 us; 1024 keys B=16 9.0 / 12.3 us; 4096 keys B=8 16.7 /
+  // 18.2 us; B=100 of 1 to 1024 keys 25.1 / 27.1 us, of 1 to 4096 keys 82.8 /
+  // 72.7 us.  The limits keep the worst case, one long sequence among short
+  // ones, at about twice the line's time.
+  const bool few = units <= 128 && head_dim <= 128;
+  p.nw = few ? 8 : kPagedLineWarps;
+  const int64_t tiles = (cap + p.nw * kPagedWarpKeys - 1) / (p.nw * kPagedWarpKeys);
+  p.cluster = 1;
+  while (p.cluster < 8 && units * p.cluster * 2 <= 128 && p.cluster < tiles) p.cluster *= 2;
+  if ((tiles + p.cluster - 1) / p.cluster > (few ? 8 : 16)) p.cluster = 0;
+  if (p.cluster) {
+    p.grid = static_cast<int>(units * p.cluster);
+    return p;
+  }
+  p.nw = kPagedLineWarps;
+  const int per_sm = head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1;  // by shared memory
+  const int64_t line = units * ((cap + kPagedLineTile - 1) / kPagedLineTile);
+  p.grid = static_cast<int>(std::min<int64_t>(line, static_cast<int64_t>(num_sms()) * per_sm));
   return p;
 }
 
@@ -767,8 +786,8 @@ int fdl_page_slots(const int32_t* lens, const int32_t* n_new, int batch, int32_t
   a.page.init(static_cast<uint32_t>(page_size));
   const int grid = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(num_sms(), (n_rows + kSlotsThreads - 1) / kSlotsThreads)));
-  page_slots_kernel<<<grid, kSlotsThreads, (2 * batch + 1) * sizeof(int32_t), reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  return launch_status();
+  return launch_after(page_slots_kernel, grid, kSlotsThreads, (2 * batch + 1) * static_cast<int>(sizeof(int32_t)),
+                      reinterpret_cast<cudaStream_t>(stream), 1, a);
 }
 
 int fdl_page_release(const uint8_t* done, int32_t* lens, int batch, int32_t* table, int64_t table_sb, int max_pages,
@@ -779,8 +798,8 @@ int fdl_page_release(const uint8_t* done, int32_t* lens, int batch, int32_t* tab
   if (!done || !lens || !count || (max_pages > 0 && !table) || (n_free > 0 && !free_pages)) return FDL_E_NULL;
   PageReleaseArgs a{done, lens, table, table_sb, free_pages, count, batch, max_pages, n_free, {}};
   a.page.init(static_cast<uint32_t>(page_size));
-  page_release_kernel<<<1, kSlotsThreads, batch * sizeof(int32_t), reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  return launch_status();
+  return launch_after(page_release_kernel, 1, kSlotsThreads, batch * static_cast<int>(sizeof(int32_t)),
+                      reinterpret_cast<cudaStream_t>(stream), 1, a);
 }
 
 int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos, const float* inv_freq, int n_freq,
@@ -812,10 +831,7 @@ int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos, const f
   const int64_t lanes = (static_cast<int64_t>(hq) + 2 * static_cast<int64_t>(hkv)) * gs;
   const int threads = static_cast<int>(std::min<int64_t>(kNrMaxThreads, (lanes + 31) / 32 * 32));
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(rows), threads, 0, s>>>(a);
-    return launch_status();
-  };
+  auto go = [&](auto kernel) { return launch_after(kernel, static_cast<unsigned>(rows), threads, 0, s, 1, a); };
   auto by_gs = [&](auto t, auto inter) {
     using T = decltype(t);
     constexpr bool kInter = decltype(inter)::value;
@@ -835,7 +851,7 @@ int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos, const f
 int64_t fdl_paged_attn_workspace_bytes(int batch, int hq, int hkv, int head_dim, int64_t max_len) {
   if (batch < 1 || hq < 1 || hkv < 1 || hq % hkv || max_len < 0) return 0;
   const PagedPlan p = paged_plan(batch, hq, hkv, head_dim, max_len);
-  if (!p.joined) return 0;
+  if (p.cluster) return 0;
   return static_cast<int64_t>(p.grid) * (2 * 8 * p.nh * (static_cast<int64_t>(head_dim) * 4 + 8) + 16);
 }
 
@@ -846,7 +862,7 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
                    fdl_stream_t stream) {
   if (dtype != FDL_BF16 && dtype != FDL_F16) return FDL_E_DTYPE;
   if (batch < 0 || batch > 65535 || hq < 1 || hq > 4096 || hkv < 1 || hq % hkv || num_pages < 0 || page_size < 1 ||
-      max_pages < 0 || table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX - kPagedTile)
+      max_pages < 0 || table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX - 1024)
     return FDL_E_SHAPE;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FDL_E_UNSUPPORTED;
   if (batch == 0) return FDL_OK;
@@ -862,7 +878,7 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
                   kv_ss * 2, kv_sh * 2, table, table_sb, lens, out, o_sb, o_sh, batch, hq, hkv, num_pages, G, HG,
                   hkv * HG, cap, {}, scale * 1.4426950408889634f, nullptr, nullptr, nullptr};
   a.page.init(static_cast<uint32_t>(page_size));
-  if (plan.joined) {
+  if (!plan.cluster) {
     if (!workspace || workspace_bytes < fdl_paged_attn_workspace_bytes(batch, hq, hkv, head_dim, cap))
       return FDL_E_WORKSPACE;
     if (!aligned16(workspace)) return FDL_E_ALIGN;
@@ -874,24 +890,28 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
   auto go = [&](auto t, auto d, auto nh) -> int {
     using T = decltype(t);
     constexpr int D = decltype(d)::value, NH = decltype(nh)::value;
-    constexpr int smem = PagedCfg<D, NH>::kSmem;
-    if (!smem_configured<paged_attn_kernel<T, D, NH>>(smem)) return FDL_E_NODEVICE;
-    paged_attn_kernel<T, D, NH><<<plan.grid, kPagedThreads, smem, s>>>(a);
-    int rc = launch_status();
-    if (rc != FDL_OK || !plan.joined) return rc;
-    // The joining kernel may start while the first one runs (it waits for its
-    // end before it reads), which hides its launch.
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(plan.grid, std::min(G, H));
-    cfg.blockDim = dim3(128);
-    cfg.stream = s;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, NH>, a, plan.grid);
-    return e == cudaSuccess ? FDL_OK : -static_cast<int>(e);
+    constexpr int smem4 = PagedCfg<D, NH, 4>::kSmem, smem8 = PagedCfg<D, NH, 8>::kSmem;
+    if constexpr ((D) < 256)
+      if (plan.cluster && plan.nw == 8) {
+        if (!smem_configured<paged_attn_kernel<T, D, NH, 8, false>>(smem8)) return FDL_E_NODEVICE;
+        return launch_after(paged_attn_kernel<T, D, NH, 8, false>, plan.grid, 256, smem8, s, plan.cluster, a);
+      }
+    if (plan.cluster) {
+      if (!smem_configured<paged_attn_kernel<T, D, NH, 4, false>>(smem4)) return FDL_E_NODEVICE;
+      return launch_after(paged_attn_kernel<T, D, NH, 4, false>, plan.grid, 128, smem4, s, plan.cluster, a);
+    }
+    if (!smem_configured<paged_attn_kernel<T, D, NH, 4, true>>(smem4)) return FDL_E_NODEVICE;
+    const int rc = launch_after(paged_attn_kernel<T, D, NH, 4, true>, plan.grid, 128, smem4, s, 1, a);
+    if (rc != FDL_OK) return rc;
+    // At most one open unit a CTA.  With few units each has many pieces, and
+    // fewer joining CTAs get more warps (one 65k-key sequence: 74 pieces a
+    // unit, joined in 2 us instead of 5 us).
+    const int64_t units = static_cast<int64_t>(batch) * a.NU;
+    const int heads = std::min(G, H);
+    if (units * 8 <= plan.grid)
+      return launch_after(paged_join_kernel<T, D, NH, true>, dim3(static_cast<unsigned>(units), heads), 512, 0, s, 1, a,
+                          plan.grid);
+    return launch_after(paged_join_kernel<T, D, NH, false>, dim3(plan.grid, heads), 128, 0, s, 1, a, plan.grid);
   };
   auto by_nh = [&](auto t, auto d) {
     if constexpr ((decltype(d)::value) < 256)

@@ -82,6 +82,8 @@ __global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_c
   // (cos, sin) of pair j, ordered so that the lanes of a head read
   // consecutive 16-byte pieces.
   __shared__ float4 s_cs[kNrMaxDim / 4];
+  await_stream();
+  release_stream();
   const int row = blockIdx.x;
   const int L = a.D / 16;        // lanes that hold elements of a head
   const int RL = a.rot / 16;     // of these, lanes that turn pairs (half layout)

@@ -91,6 +91,8 @@ __global__ void __launch_bounds__(kSlotsThreads) page_slots_kernel(const __grid_
   int32_t* s_at = s_buf + a.B + 1;  // [B]: order of b's first new page, -1 = refused
   __shared__ SlotSums sh_scan[kSlotsThreads / 32];
   __shared__ int sh_last, sh_taken;
+  await_stream();
+  release_stream();
   const int count = min(max(a.count[0], 0), a.n_free);
   if (threadIdx.x == 0) sh_taken = 0;
   const int per = (a.B + kSlotsThreads - 1) / kSlotsThreads;
@@ -192,6 +194,8 @@ __global__ void __launch_bounds__(kSlotsThreads) page_release_kernel(const __gri
   extern __shared__ int32_t s_n[];  // [B] pages of the row, then their order
   __shared__ SlotSums sh_scan[kSlotsThreads / 32];
   __shared__ int64_t sh_total;
+  await_stream();
+  release_stream();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int b = warp; b < a.B; b += kSlotsThreads / 32) {
     int n = -1;

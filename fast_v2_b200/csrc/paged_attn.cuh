@@ -11,14 +11,19 @@
 // every SM, whatever the lengths.
 //
 // Unit = (sequence, KV head, group of 8 * NH query heads); its keys come in
-// tiles of 64.  The tiles of all units form one line, and each CTA of a grid
-// that fits the GPU takes an equal piece of it (found with one scan of the
-// lengths, on the device: lengths may change under a captured graph).  A unit
-// that lies in one piece is finished by its CTA; the pieces of the others go
-// to the workspace -- at most two a CTA, so the workspace does not grow with
-// the batch -- and a second kernel joins them in order.  Where the longest
-// possible sequence is short, a CTA takes a whole unit and there is nothing
-// to join.
+// tiles of 16 per warp.  Two ways to share the units out (chosen by
+// paged_plan on sizes alone):
+//   line     The tiles of all units form one line, and each CTA of a grid that
+//            fits the GPU takes an equal piece of it (found with one scan of
+//            the lengths, on the device: lengths may change under a captured
+//            graph).  A unit that lies in one piece is finished by its CTA;
+//            the pieces of the others go to the workspace -- at most two a
+//            CTA, so it does not grow with the batch -- and a second kernel
+//            joins them in order.
+//   cluster  A thread-block cluster takes a unit, its CTAs equal parts of the
+//            unit's tiles, joined through distributed shared memory: one
+//            launch, no workspace.  For short caches, where the scan and the
+//            second kernel cost more than an uneven share.
 //
 // Within a CTA every warp takes 16 keys of a tile and runs on its own: its
 // rows arrive by cp.async in a ring of its own, no barrier between warps
@@ -52,29 +57,25 @@ struct PagedAttnArgs {
   int cap;                  // keys the table can name
   FastDiv page;
   float scale_log2;
-  // joining (null: every CTA takes one whole unit)
+  // line
   float* part_o;            // [2 grid, 8 NH, D] sums relative to the piece's reference
   float2* part_ml;          // [2 grid, 8 NH] (reference, sum of p)
   int4* desc;               // [grid] (sequence, unit of it) whose first piece ends the CTA's part of the line, or -1;
                             // state of the CTA's first piece: 0 starts a unit, 1 middle of one, 2 end of one
 };
 
-constexpr int kPagedWarps = 4;
-constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kPagedWarpKeys = 16;
-constexpr int kPagedTile = kPagedWarps * kPagedWarpKeys;
+constexpr int kPagedLineWarps = 4;
+constexpr int kPagedLineTile = kPagedLineWarps * kPagedWarpKeys;
 // A score may pass the running reference by 2^8 before the sums are scaled
 // down to a new one (p <= 256 in either 16-bit type).
 constexpr float kPagedSlack = 8.f;
 
-template <int D, int NH>
+template <int D, int NH, int NW>
 struct PagedCfg {
-  static constexpr int kStages = D == 64 ? 4 : D == 128 ? (NH == 1 ? 3 : 2) : 2;
-  static constexpr int kStage = 2 * kPagedWarpKeys * D * 2;  // bytes: K rows, V rows
-  static constexpr int kRing = kPagedWarps * kStages * kStage;
-  static constexpr int kMergeRow = D + 4;  // floats: the four heads of a lane group land in different banks
-  static constexpr int kMerge = kPagedWarps * 8 * NH * kMergeRow * 4;
-  static constexpr int kSmem = kRing + kMerge;
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStage = 2 * kPagedWarpKeys * D * 2;  // bytes of a warp's tile: K rows, V rows
+  static constexpr int kSmem = NW * kStages * kStage;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -135,53 +136,94 @@ __device__ __forceinline__ int paged_div(const FastDiv& f, int n) {
   return static_cast<int>(hi >> 32);
 }
 
-// A place on the line of tiles.
+// A place on the line of tiles of NW * 16 keys.
+template <int TILE>
 struct PagedPos {
-  int b, n;      // sequence, unit of the sequence
-  int t, nt;     // tile of the unit, tiles of a unit of b
+  int b, kh, hg;  // sequence, KV head, group of its query heads
+  int t, nt;      // tile of the unit, tiles of a unit of b
   int len;
+  __device__ __forceinline__ void unit(const PagedAttnArgs& a, int n) {
+    kh = n / a.HG;
+    hg = n - kh * a.HG;
+  }
   __device__ __forceinline__ void next(const PagedAttnArgs& a) {
     if (++t < nt) return;
     t = 0;
-    if (++n < a.NU) return;
-    n = 0;
+    if (++hg < a.HG) return;
+    hg = 0;
+    if (++kh < a.hkv) return;
+    kh = 0;
     for (++b; b < a.B; ++b) {
       len = paged_len(a, b);
-      nt = (len + kPagedTile - 1) / kPagedTile;
+      nt = (len + TILE - 1) / TILE;
       if (nt > 0) return;
     }
   }
 };
 
-template <typename T, int D, int NH>
-__global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
-  using Cfg = PagedCfg<D, NH>;
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 16 bytes (8 bytes) of the shared memory of CTA `rank` of the cluster, at
+// this CTA's address.
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+  uint32_t at;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr, uint32_t rank) {
+  uint32_t at;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
+template <typename T, int D, int NH, int NW, bool LINE>
+__global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+  using Cfg = PagedCfg<D, NH, NW>;
+  constexpr int kThreads = NW * 32, kTile = NW * kPagedWarpKeys;
   constexpr int kStages = Cfg::kStages, kChunks = D / 8, kRowB = D * 2, H = 8 * NH;
   constexpr int kLoads = kPagedWarpKeys * kChunks / 32;  // 16-byte pieces of K (and of V) a lane and tile
   extern __shared__ __align__(128) char smem[];
-  __shared__ int s_mask[kPagedWarps][kStages];
-  __shared__ float2 s_ml[kPagedWarps][H];
+  __shared__ int s_mask[NW][kStages];
+  __shared__ float2 s_ml[NW][H];
+  __shared__ float2 s_cta[H];  // cluster: (reference, sum) of this CTA
   __shared__ int s_pos[4];
-  __shared__ long long s_scan[kPagedWarps];
+  __shared__ long long s_scan[NW];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c4 = lane & 3;
-  float* s_merge = reinterpret_cast<float*>(smem + Cfg::kRing);
   const uint32_t ring = smem_addr(smem) + warp * kStages * Cfg::kStage;
   T* const out = static_cast<T*>(a.out);
 
   // ---- this CTA's piece of the line
-  PagedPos p{};
+  PagedPos<kTile> p{};
   int left;  // tiles
-  bool joined = a.part_o != nullptr;
-  if (joined) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int per = (a.B + kPagedThreads - 1) / kPagedThreads;
+  await_stream();
+  release_stream();
+  if constexpr (LINE) {
+    const int per = (a.B + kThreads - 1) / kThreads;
     const int b0 = threadIdx.x * per, b1 = min(a.B, b0 + per);
     long long sum = 0;
     for (int b = b0; b < b1; ++b) {
       const int raw = a.lens[b];
       if (blockIdx.x == 0 && (raw < 0 || raw > a.cap)) report(FDL_DEV_LENGTH, b);
-      sum += (min(max(raw, 0), a.cap) + kPagedTile - 1) / kPagedTile;
+      sum += (min(max(raw, 0), a.cap) + kTile - 1) / kTile;
     }
     long long incl = sum;
 #pragma unroll
@@ -193,7 +235,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
     __syncthreads();
     long long total = 0;
 #pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) {
+    for (int w = 0; w < NW; ++w) {
       if (w < warp) incl += s_scan[w];
       total += s_scan[w];
     }
@@ -210,7 +252,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
     long long at = (incl - sum) * a.NU;
     if (left > 0 && first >= at && first < incl * a.NU) {
       for (int b = b0; b < b1; ++b) {
-        const int len = paged_len(a, b), nt = (len + kPagedTile - 1) / kPagedTile;
+        const int len = paged_len(a, b), nt = (len + kTile - 1) / kTile;
         const long long mine = static_cast<long long>(nt) * a.NU;
         if (first < at + mine) {
           const int local = static_cast<int>(first - at);
@@ -226,7 +268,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
     // Sequences without keys: shared out over the grid.
     for (int b = blockIdx.x; b < a.B; b += gridDim.x)
       if (paged_len(a, b) == 0)
-        for (int i = threadIdx.x; i < a.hq * kChunks; i += kPagedThreads)
+        for (int i = threadIdx.x; i < a.hq * kChunks; i += kThreads)
           *reinterpret_cast<uint4*>(out + b * a.o_sb + (i / kChunks) * a.o_sh + (i % kChunks) * 8) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     if (left == 0) {
@@ -234,32 +276,36 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
       return;
     }
     p.b = s_pos[0];
-    p.n = s_pos[1];
+    p.unit(a, s_pos[1]);
     p.t = s_pos[2];
     p.len = s_pos[3];
   } else {
-    p.b = blockIdx.x / a.NU;
-    p.n = blockIdx.x % a.NU;
+    const uint32_t ranks = cluster_size(), rank = cluster_rank(), unit = blockIdx.x / ranks;
+    p.b = unit / a.NU;
+    p.unit(a, unit % a.NU);
     const int raw = a.lens[p.b];
-    if (p.n == 0 && threadIdx.x == 0 && (raw < 0 || raw > a.cap)) report(FDL_DEV_LENGTH, p.b);
-    p.len = paged_len(a, p.b);
-    left = (p.len + kPagedTile - 1) / kPagedTile;
-    if (left == 0) {
-      const int h0 = (p.n / a.HG) * a.G + (p.n % a.HG) * H, hn = min(H, a.G - (p.n % a.HG) * H);
-      for (int i = threadIdx.x; i < hn * kChunks; i += kPagedThreads)
-        *reinterpret_cast<uint4*>(out + p.b * a.o_sb + (h0 + i / kChunks) * a.o_sh + (i % kChunks) * 8) =
-            make_uint4(0, 0, 0, 0);
+    if (rank == 0 && unit % a.NU == 0 && threadIdx.x == 0 && (raw < 0 || raw > a.cap)) report(FDL_DEV_LENGTH, p.b);
+    p.len = min(max(raw, 0), a.cap);
+    const int nt = (p.len + kTile - 1) / kTile;
+    if (nt == 0) {  // no CTA of the cluster goes on
+      const int h0 = p.kh * a.G + p.hg * H, hn = min(H, a.G - p.hg * H);
+      if (rank == 0)
+        for (int i = threadIdx.x; i < hn * kChunks; i += kThreads)
+          *reinterpret_cast<uint4*>(out + p.b * a.o_sb + (h0 + i / kChunks) * a.o_sh + (i % kChunks) * 8) =
+              make_uint4(0, 0, 0, 0);
       return;
     }
+    p.t = nt * rank / ranks;
+    left = nt * (rank + 1) / ranks - p.t;
   }
-  p.nt = (p.len + kPagedTile - 1) / kPagedTile;
-  // 0: the first piece starts its unit
+  p.nt = (p.len + kTile - 1) / kTile;
+  // line: 0 this CTA's first piece starts its unit, 1 lies inside, 2 ends it
   int state = p.t == 0 ? 0 : (p.t + left >= p.nt ? 2 : 1);
   const int first_state = state;
 
   // ---- loads: the warp's 16 rows of tile `w`, with the pages looked up one tile ahead
   constexpr int kRows = 32 / kChunks;  // rows a warp-wide copy covers (D = 64: 4, 128: 2, 256: 1)
-  PagedPos w = p;  // next tile to load
+  PagedPos<kTile> w = p;  // next tile to load
   int w_left = left;
   const bool whole = a.page.d % kPagedWarpKeys == 0;  // the 16 keys lie in one page
   const int64_t lane_src = static_cast<int64_t>(lane / kChunks) * a.ss + (lane % kChunks) * 16;
@@ -282,7 +328,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
   int page = 0, in_page = 0;
   auto look_up = [&]() {  // the page of this lane's key of tile w
     if (w_left > 0) {
-      const int key = w.t * kPagedTile + warp * kPagedWarpKeys + (whole ? 0 : lane & 15);
+      const int key = w.t * kTile + warp * kPagedWarpKeys + (whole ? 0 : lane & 15);
       if (key < w.len) {
         const int i = paged_div(a.page, key);
         in_page = key - i * static_cast<int>(a.page.d);
@@ -293,11 +339,11 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
   int fill = 0;
   auto load = [&]() {
     if (w_left > 0) {
-      const int n = w.len - w.t * kPagedTile - warp * kPagedWarpKeys;  // keys from the warp's first on
+      const int n = w.len - w.t * kTile - warp * kPagedWarpKeys;  // keys from the warp's first on
       if (n > 0) {
         const bool bad = static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_pages);
         const int64_t off = static_cast<int64_t>(page) * a.sp + static_cast<int64_t>(in_page) * a.ss +
-                            static_cast<int64_t>(w.n / a.HG) * a.sh;
+                            static_cast<int64_t>(w.kh) * a.sh;
         const uint32_t dst = ring + fill * Cfg::kStage;
         if (whole && n >= kPagedWarpKeys && !bad) {
           if (lane == 0) s_mask[warp][fill] = 0xffff;
@@ -341,33 +387,97 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
   uint32_t qf[NH][D / 16][2];
   float o[NH][D / 16][4];
   float m[NH][2], l[NH][2];
-  int use = 0;
-  bool fresh = true;
-  while (left > 0) {
-    const int kh = p.n / a.HG, h0 = kh * a.G + (p.n % a.HG) * H, hn = min(H, a.G - (p.n % a.HG) * H);
-    if (fresh) {
-      fresh = false;
-      const T* q = static_cast<const T*>(a.q) + p.b * a.q_sb + h0 * a.q_sh;
+  auto load_q = [&]() {  // the query heads of p's unit
+    const int h0 = p.kh * a.G + p.hg * H, hn = min(H, a.G - p.hg * H);
+    const T* q = static_cast<const T*>(a.q) + p.b * a.q_sb + h0 * a.q_sh;
 #pragma unroll
-      for (int x = 0; x < NH; ++x) {
-        const int hh = x * 8 + g;
+    for (int x = 0; x < NH; ++x) {
+      const int hh = x * 8 + g;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
+      for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            qf[x][kk][e] = hh < hn ? *reinterpret_cast<const uint32_t*>(q + hh * a.q_sh + kk * 16 + e * 8 + c4 * 2) : 0u;
+        for (int e = 0; e < 2; ++e)
+          qf[x][kk][e] = hh < hn ? *reinterpret_cast<const uint32_t*>(q + hh * a.q_sh + kk * 16 + e * 8 + c4 * 2) : 0u;
+    }
+  };
+  auto clear = [&]() {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[x][kk][e] = 0.f;
-        }
-        m[x][0] = m[x][1] = -INFINITY;
-        l[x][0] = l[x][1] = 0.f;
+    for (int x = 0; x < NH; ++x) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[x][kk][e] = 0.f;
+      m[x][0] = m[x][1] = -INFINITY;
+      l[x][0] = l[x][1] = 0.f;
+    }
+  };
+  // The warp's state goes to its part of `to` ([H, D] floats; the 8-float
+  // pieces of a head are exchanged so that the four heads that a warp writes
+  // at a time lie in different banks).
+  auto put_state = [&](float* to) {
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], off);
+      if (g == 0) {
+        s_ml[warp][x * 8 + c4 * 2] = make_float2(m[x][0], l[x][0]);
+        s_ml[warp][x * 8 + c4 * 2 + 1] = make_float2(m[x][1], l[x][1]);
+      }
+      float* mo = to + (x * 8 + c4 * 2) * D;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const int d0 = ((kk * 2) ^ c4) * 8 + g, d1 = ((kk * 2 + 1) ^ c4) * 8 + g;
+        mo[d0] = o[x][kk][0];
+        mo[D + d0] = o[x][kk][1];
+        mo[d1] = o[x][kk][2];
+        mo[D + d1] = o[x][kk][3];
       }
     }
+  };
+  // Eight elements of head hh, summed over the warps' states (`stride` floats
+  // apart) relative to the largest reference M; L is the sum of p.
+  auto take_state = [&](const float* from, int stride, int hh, int ch, float (&acc)[8], float& M, float& L) {
+    M = -INFINITY;
+    L = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) M = fmaxf(M, s_ml[x][hh].x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float2 ml = s_ml[x][hh];
+      const float f = ex2(ml.x - ref);
+      L = fmaf(ml.y, f, L);
+      const float4* src = reinterpret_cast<const float4*>(from + x * stride + hh * D + ((ch ^ ((hh >> 1) & 3)) * 8));
+      const float4 u0 = src[0], u1 = src[1];
+      acc[0] = fmaf(u0.x, f, acc[0]);
+      acc[1] = fmaf(u0.y, f, acc[1]);
+      acc[2] = fmaf(u0.z, f, acc[2]);
+      acc[3] = fmaf(u0.w, f, acc[3]);
+      acc[4] = fmaf(u1.x, f, acc[4]);
+      acc[5] = fmaf(u1.y, f, acc[5]);
+      acc[6] = fmaf(u1.z, f, acc[6]);
+      acc[7] = fmaf(u1.w, f, acc[7]);
+    }
+  };
+  auto finish = [&](int b, int h, int ch, float (&acc)[8], float L) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= inv;
+    *reinterpret_cast<uint4*>(out + b * a.o_sb + h * a.o_sh + ch * 8) = pack8<T>(acc);
+  };
+  load_q();
+  clear();
+  int use = 0;
+  while (left > 0) {
     __syncwarp();  // the slot that is loaded next has been read
     load();
     cp_wait<kStages - 1>();
     __syncwarp();
-    if (p.t * kPagedTile + warp * kPagedWarpKeys < p.len) {
+    if (p.t * kTile + warp * kPagedWarpKeys < p.len) {
       const uint32_t slot = ring + use * Cfg::kStage;
       const unsigned mask = s_mask[warp][use];
       float s[NH][2][4];
@@ -433,111 +543,169 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const __grid_
         for (int x = 0; x < NH; ++x) mma16816<T>(o[x][kk], f, pf[x][0], pf[x][1]);
       }
     }
-    use = use + 1 == kStages ? 0 : use + 1;
     --left;
-    const bool ends = p.t + 1 == p.nt;
-    if (ends || left == 0) {
-      // ---- join the warps; finish the unit, or leave the piece in the workspace
-#pragma unroll
-      for (int x = 0; x < NH; ++x) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], off);
-        if (g == 0) {
-          s_ml[warp][x * 8 + c4 * 2] = make_float2(m[x][0], l[x][0]);
-          s_ml[warp][x * 8 + c4 * 2 + 1] = make_float2(m[x][1], l[x][1]);
-        }
-        float* mo = s_merge + (warp * H + x * 8 + c4 * 2) * Cfg::kMergeRow;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          mo[kk * 16 + g] = o[x][kk][0];
-          mo[Cfg::kMergeRow + kk * 16 + g] = o[x][kk][1];
-          mo[kk * 16 + g + 8] = o[x][kk][2];
-          mo[Cfg::kMergeRow + kk * 16 + g + 8] = o[x][kk][3];
-        }
-      }
-      __syncthreads();
-      const bool all = state == 0 && ends;
-      const int piece = blockIdx.x * 2 + (state == 0 ? 1 : 0);
-      for (int i = threadIdx.x; i < hn * kChunks; i += kPagedThreads) {
-        const int hh = i / kChunks, ch = i % kChunks;
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int x = 0; x < kPagedWarps; ++x) M = fmaxf(M, s_ml[x][hh].x);
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll
-        for (int x = 0; x < kPagedWarps; ++x) {
-          const float2 ml = s_ml[x][hh];
-          const float f = ex2(ml.x - ref);
-          L = fmaf(ml.y, f, L);
-          const float4* src = reinterpret_cast<const float4*>(s_merge + (x * H + hh) * Cfg::kMergeRow + ch * 8);
-          const float4 u0 = src[0], u1 = src[1];
-          acc[0] = fmaf(u0.x, f, acc[0]);
-          acc[1] = fmaf(u0.y, f, acc[1]);
-          acc[2] = fmaf(u0.z, f, acc[2]);
-          acc[3] = fmaf(u0.w, f, acc[3]);
-          acc[4] = fmaf(u1.x, f, acc[4]);
-          acc[5] = fmaf(u1.y, f, acc[5]);
-          acc[6] = fmaf(u1.z, f, acc[6]);
-          acc[7] = fmaf(u1.w, f, acc[7]);
-        }
-        if (all) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] *= inv;
-          *reinterpret_cast<uint4*>(out + p.b * a.o_sb + (h0 + hh) * a.o_sh + ch * 8) = pack8<T>(acc);
-        } else {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(piece) * H + hh) * D + ch * 8);
-          dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-          dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-          if (ch == 0) a.part_ml[piece * H + hh] = make_float2(M, L);
-        }
-      }
-      if (joined && left == 0 && threadIdx.x == 0)
-        a.desc[blockIdx.x] = make_int4(state == 0 && !ends ? p.b : -1, p.n, first_state, 0);
-      __syncthreads();  // s_merge and s_ml are free again
-      fresh = true;
-      state = 0;
-    }
+    const PagedPos<kTile> was = p;
     if (left > 0) p.next(a);
+    if constexpr (LINE) {
+      const bool ends = was.t + 1 == was.nt;
+      if (ends || left == 0) {
+        // ---- finish the unit, or leave the piece in the workspace.  The
+        // slot that was read last is the warp's room: nothing is loaded into
+        // it before the next tile.
+        if (left > 0) load_q();  // on its way while the warps are joined
+        const float* room = reinterpret_cast<const float*>(smem + use * Cfg::kStage);
+        put_state(const_cast<float*>(room) + warp * (kStages * Cfg::kStage / 4));
+        __syncthreads();
+        const bool all = state == 0 && ends;
+        const int piece = blockIdx.x * 2 + (state == 0 ? 1 : 0);
+        const int h0 = was.kh * a.G + was.hg * H, hn = min(H, a.G - was.hg * H);
+        for (int i = threadIdx.x; i < hn * kChunks; i += kThreads) {
+          const int hh = i / kChunks, ch = i % kChunks;
+          float acc[8], M, L;
+          take_state(room, kStages * Cfg::kStage / 4, hh, ch, acc, M, L);
+          if (all) {
+            finish(was.b, h0 + hh, ch, acc, L);
+          } else {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(piece) * H + hh) * D + ch * 8);
+            dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            if (ch == 0) a.part_ml[piece * H + hh] = make_float2(M, L);
+          }
+        }
+        if (left == 0 && threadIdx.x == 0)
+          a.desc[blockIdx.x] = make_int4(state == 0 && !ends ? was.b : -1, was.kh * a.HG + was.hg, first_state, 0);
+        __syncthreads();  // the room and s_ml are free again
+        clear();
+        state = 0;
+      }
+    }
+    use = use + 1 == kStages ? 0 : use + 1;
   }
   cp_wait<0>();
+  if constexpr (!LINE) {
+    __syncthreads();  // the whole ring is room
+    float* room = reinterpret_cast<float*>(smem);
+    put_state(room + warp * H * D);
+    __syncthreads();
+    const uint32_t ranks = cluster_size();
+    const int h0 = p.kh * a.G + p.hg * H, hn = min(H, a.G - p.hg * H);
+    if (ranks == 1) {
+      for (int i = threadIdx.x; i < hn * kChunks; i += kThreads) {
+        float acc[8], M, L;
+        take_state(room, H * D, i / kChunks, i % kChunks, acc, M, L);
+        finish(p.b, h0 + i / kChunks, i % kChunks, acc, L);
+      }
+      return;
+    }
+    // This CTA's sums, in the room of warp 0 (a thread overwrites only what it
+    // alone has read), then all CTAs' for a share of the outputs each.
+    for (int i = threadIdx.x; i < H * kChunks; i += kThreads) {
+      const int hh = i / kChunks, ch = i % kChunks;
+      float acc[8], M, L;
+      take_state(room, H * D, hh, ch, acc, M, L);
+      float4* dst = reinterpret_cast<float4*>(room + hh * D + ((ch ^ ((hh >> 1) & 3)) * 8));
+      dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (ch == 0) s_cta[hh] = make_float2(M, L);
+    }
+    cluster_sync();
+    for (int i = cluster_rank() * kThreads + threadIdx.x; i < hn * kChunks; i += ranks * kThreads) {
+      const int hh = i / kChunks, ch = i % kChunks;
+      float acc[8], M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+      for (uint32_t r = 0; r < ranks; ++r) M = fmaxf(M, ld_cluster2(smem_addr(&s_cta[hh]), r).x);
+      const float ref = M == -INFINITY ? 0.f : M;
+      const uint32_t src = smem_addr(room + hh * D + ((ch ^ ((hh >> 1) & 3)) * 8));
+      for (uint32_t r = 0; r < ranks; ++r) {
+        const float2 ml = ld_cluster2(smem_addr(&s_cta[hh]), r);
+        const float4 u0 = ld_cluster4(src, r), u1 = ld_cluster4(src + 16, r);
+        const float f = ex2(ml.x - ref);
+        L = fmaf(ml.y, f, L);
+        acc[0] = fmaf(u0.x, f, acc[0]);
+        acc[1] = fmaf(u0.y, f, acc[1]);
+        acc[2] = fmaf(u0.z, f, acc[2]);
+        acc[3] = fmaf(u0.w, f, acc[3]);
+        acc[4] = fmaf(u1.x, f, acc[4]);
+        acc[5] = fmaf(u1.y, f, acc[5]);
+        acc[6] = fmaf(u1.z, f, acc[6]);
+        acc[7] = fmaf(u1.w, f, acc[7]);
+      }
+      finish(p.b, h0 + hh, ch, acc, L);
+    }
+    cluster_sync();  // no CTA leaves while its shared memory is read
+  }
 }
 
-// Joins the pieces of the units that lie on more than one CTA: CTA (c, h)
-// takes query head h of the unit whose first piece ends CTA c's part of the
-// line; its other pieces are the first ones of the CTAs behind c, up to the
-// one that ends the unit.  Warps take pieces in turn and are joined in order.
-template <typename T, int D, int NH>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int grid) {
-  constexpr int H = 8 * NH, E = D / 32;
-  __shared__ float s_o[4][D];
-  __shared__ float2 s_ml[4];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, hh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int4 d = a.desc[c];
-  if (d.x < 0) return;
+// Joins the pieces of the units that lie on more than one CTA.  CTA (i, h)
+// takes query head h of a unit that CTA c of the line leaves open -- c = i, or
+// with few units the i-th such CTA: its pieces are the last one of CTA c and
+// the first ones of the CTAs behind c, up to the one that ends the unit.  The
+// warps take pieces in turn and are joined in order.
+template <typename T, int D, int NH, bool FEW>
+__global__ void __launch_bounds__(FEW ? 512 : 128) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, int grid) {
+  constexpr int NW = FEW ? 16 : 4, H = 8 * NH, E = D / 32;
+  __shared__ float s_o[NW][D];
+  __shared__ float2 s_ml[NW];
+  await_stream();
+  release_stream();
+  const int hh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int c, last = -1;
+  int4 d;
+  if constexpr (FEW) {
+    // the i-th CTA that leaves a unit open, and the next one that ends one:
+    // a warp reads all descriptors, eight a lane at a time
+    c = -1;
+    d = make_int4(-1, 0, 0, 0);
+    int want = blockIdx.x;  // open units to pass
+    for (int i0 = 0; i0 < grid && last < 0; i0 += 256) {
+      int4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * 32 + lane;
+        v[u] = i < grid ? a.desc[i] : make_int4(-1, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        unsigned end = __ballot_sync(0xffffffffu, v[u].z == 2), open = __ballot_sync(0xffffffffu, v[u].x >= 0);
+        if (last >= 0) continue;
+        if (c < 0) {
+          if (want >= __popc(open)) {
+            want -= __popc(open);
+            continue;
+          }
+          for (; want > 0; --want) open &= open - 1;
+          const int at = __ffs(open) - 1;
+          c = i0 + u * 32 + at;
+          d.x = __shfl_sync(0xffffffffu, v[u].x, at);
+          d.y = __shfl_sync(0xffffffffu, v[u].y, at);
+          end &= at == 31 ? 0u : 0xffffffffu << (at + 1);
+        }
+        if (end) last = i0 + u * 32 + __ffs(end) - 1;
+      }
+    }
+  } else {
+    c = blockIdx.x;
+    d = a.desc[c];
+    if (d.x < 0) return;
+    for (int i0 = c + 1; i0 < grid && last < 0; i0 += 32) {
+      const unsigned end = __ballot_sync(0xffffffffu, i0 + lane < grid && a.desc[i0 + lane].z == 2);
+      if (end) last = i0 + __ffs(end) - 1;
+    }
+  }
+  if (last < 0) return;
   const int g0 = (d.y % a.HG) * H;
   if (hh >= min(H, a.G - g0)) return;
-  // the piece that ends the unit: the first CTA behind c in that state
-  int last = c;
-  for (int i0 = c + 1; i0 < grid; i0 += 32) {
-    const unsigned end = __ballot_sync(0xffffffffu, i0 + lane < grid && a.desc[i0 + lane].z == 2);
-    last = end ? i0 + __ffs(end) - 1 : min(i0 + 31, grid - 1);
-    if (end) break;
-  }
   // Each warp keeps a reference of its own, four pieces at a time.
   float acc[E], L = 0.f, M = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int i0 = c + warp; i0 <= last; i0 += 16) {
+  for (int i0 = c + warp; i0 <= last; i0 += 4 * NW) {
     float2 ml[4];
     float x[4][E];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * 4;
+      const int i = i0 + u * NW;
       ml[u] = make_float2(-INFINITY, 0.f);
       if (i <= last) {
         const int slot = (i * 2 + (i == c)) * H + hh;
@@ -569,17 +737,22 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   for (int e = 0; e < E; ++e) s_o[warp][e * 32 + lane] = acc[e];
   if (lane == 0) s_ml[warp] = make_float2(M, L);
   __syncthreads();
-  const float2 m0 = s_ml[0], m1 = s_ml[1], m2 = s_ml[2], m3 = s_ml[3];
-  const float top = fmaxf(fmaxf(m0.x, m1.x), fmaxf(m2.x, m3.x));
+  float top = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) top = fmaxf(top, s_ml[w].x);
   const float ref = top == -INFINITY ? 0.f : top;
-  const float f[4] = {ex2(m0.x - ref), ex2(m1.x - ref), ex2(m2.x - ref), ex2(m3.x - ref)};
-  const float l = m0.y * f[0] + m1.y * f[1] + m2.y * f[2] + m3.y * f[3];
+  float f[NW];
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    f[w] = ex2(s_ml[w].x - ref);
+    l = fmaf(s_ml[w].y, f[w], l);
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* out = static_cast<T*>(a.out) + d.x * a.o_sb + ((d.y / a.HG) * a.G + g0 + hh) * a.o_sh;
-  for (int i = threadIdx.x; i < D / 2; i += 128) {
+  for (int i = threadIdx.x; i < D / 2; i += NW * 32) {
     float x0 = 0.f, x1 = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       x0 = fmaf(s_o[w][2 * i], f[w], x0);
       x1 = fmaf(s_o[w][2 * i + 1], f[w], x1);
     }
