@@ -81,38 +81,8 @@ inline int pick_vec(std::initializer_list<uint64_t> vals) {
   return v;
 }
 
-// Programmatic dependent launch: a kernel launched by launch_after() may start
-// before the kernel ahead of it in the stream has ended, so every CTA calls
-// await_stream() before it touches global memory; it returns when that kernel
-// has ended and its writes are visible.  (Every CTA has to call it: a kernel
-// counts as ended when its CTAs have, and the next one waits for no other.)
-// release_stream() lets the next kernel of the stream be set up from then on.
-__device__ __forceinline__ void await_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void release_stream() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 inline int launch_status() {
   cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? FDL_OK : -static_cast<int>(e);
-}
-
-// Launches with await_stream() semantics; cluster: CTAs a cluster along x.
-template <typename... P, typename... A>
-inline int launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, int cluster,
-                        const A&... args) {
-  cudaLaunchAttribute at[2]{};
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = cluster;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
   return e == cudaSuccess ? FDL_OK : -static_cast<int>(e);
 }
 

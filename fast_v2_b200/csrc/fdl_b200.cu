@@ -936,10 +936,17 @@ int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int voc
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == FDL_F32 ? 4 : 2)) return FDL_E_ALIGN;
   TokScoreArgs a{logits, row_stride, vocab, targets, logprob, entropy, top, top_logprob, top_token};
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == FDL_BF16) token_scores_kernel<__nv_bfloat16><<<rows, kTokThreads, 0, s>>>(a);
-  else if (dtype == FDL_F16) token_scores_kernel<__half><<<rows, kTokThreads, 0, s>>>(a);
-  else token_scores_kernel<float><<<rows, kTokThreads, 0, s>>>(a);
-  return launch_status();
+  // CTAs a row: enough to fill the GPU (three a SM) with few rows, each with
+  // at least one vector a thread.
+  const int64_t vectors = static_cast<int64_t>(vocab) * (dtype == FDL_F32 ? 4 : 2) / 16;
+  int cluster = 1;
+  while (cluster < 8 && static_cast<int64_t>(rows) * cluster < 3ll * num_sms() && vectors >= 2ll * cluster * kTokThreads)
+    cluster *= 2;
+  if (static_cast<int64_t>(rows) * cluster > INT32_MAX) return FDL_E_SHAPE;
+  auto go = [&](auto kernel) { return launch_after(kernel, rows * cluster, kTokThreads, 0, s, cluster, a); };
+  return dtype == FDL_BF16  ? go(token_scores_kernel<__nv_bfloat16>)
+         : dtype == FDL_F16 ? go(token_scores_kernel<__half>)
+                            : go(token_scores_kernel<float>);
 }
 
 int fdl_last_device_error(int32_t* code, int64_t* info) {

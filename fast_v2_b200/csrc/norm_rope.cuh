@@ -19,6 +19,7 @@
 // are in flight before the row's cos / sin table is computed.
 #pragma once
 #include "common.cuh"
+#include "device_util.cuh"
 
 namespace fdl {
 
@@ -42,40 +43,6 @@ struct NormRopeArgs {
   float eps, scale;
   int rows, hq, hkv, D, rot;
 };
-
-template <typename T> struct Pack2;
-template <> struct Pack2<__nv_bfloat16> {
-  static __device__ __forceinline__ float2 to(uint32_t u) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  }
-  static __device__ __forceinline__ uint32_t from(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-};
-template <> struct Pack2<__half> {
-  static __device__ __forceinline__ float2 to(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
-  static __device__ __forceinline__ uint32_t from(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-};
-
-template <typename T>
-__device__ __forceinline__ void unpack8(uint4 u, float* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = Pack2<T>::to(w[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  return make_uint4(Pack2<T>::from(f[0], f[1]), Pack2<T>::from(f[2], f[3]), Pack2<T>::from(f[4], f[5]),
-                    Pack2<T>::from(f[6], f[7]));
-}
 
 template <typename T, int GS, bool INTER>
 __global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {

@@ -20,6 +20,7 @@
 // last writes them (a ticket next to the count, left at zero).
 #pragma once
 #include "common.cuh"
+#include "device_util.cuh"
 
 namespace fdl {
 

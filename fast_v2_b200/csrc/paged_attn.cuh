@@ -37,7 +37,7 @@
 #include <type_traits>
 
 #include "common.cuh"
-#include "norm_rope.cuh"
+#include "device_util.cuh"
 
 namespace fdl {
 
@@ -78,8 +78,6 @@ struct PagedCfg {
   static constexpr int kSmem = NW * kStages * kStage;
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const char* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -119,12 +117,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) { return min(max(a.lens[b], 0), a.cap); }
 
 // n / f.d for n < 2^31 (FastDiv::div with the 32-bit halves of the product
@@ -160,39 +152,6 @@ struct PagedPos {
     }
   }
 };
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// 16 bytes (8 bytes) of the shared memory of CTA `rank` of the cluster, at
-// this CTA's address.
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
-  uint32_t at;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(at)
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 ld_cluster2(uint32_t addr, uint32_t rank) {
-  uint32_t at;
-  float2 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-  return v;
-}
 
 template <typename T, int D, int NH, int NW, bool LINE>
 __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {

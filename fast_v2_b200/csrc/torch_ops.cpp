@@ -7,9 +7,11 @@
 // flash_attn_with_kvcache in utils/attention_backends.py:73-120.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <tuple>
 #include <vector>
 
 #include "../../include/fdl_kvcache.h"
@@ -762,7 +764,7 @@ void paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
                                                           as_int(hkv, "hkv"), as_int(D, "D"),
                                                           block_table.size(1) * page);
   Tensor ws;
-  if (ws_bytes > 0) ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+  if (ws_bytes > 0) ws = at::detail::empty_cuda({ws_bytes}, at::kByte, q.device(), std::nullopt);
   check_rc(fdl_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
                           k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), as_int(k_pages.size(0), "num_pages"),
                           as_int(page, "page_size"), block_table.data_ptr<int32_t>(), table_stride(block_table),
@@ -773,36 +775,35 @@ void paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
            "paged_decode_attn");
 }
 
-void token_logprobs(const Tensor& logits, const Tensor& targets, const Tensor& logprob, const Tensor& entropy,
-                    const std::optional<Tensor>& top_logprob, const std::optional<Tensor>& top_token) {
+// Returns (logprob [rows], entropy [rows], top_logprob [rows, top], top_token
+// [rows, top]); the outputs come from torch's caching allocator.
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& targets, int64_t top) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
               "fdl.token_logprobs: logits must be a CUDA [rows, vocab] tensor with unit inner stride");
   const int64_t rows = logits.size(0), V = logits.size(1);
   check_i64(targets, logits, rows, "targets");
-  TORCH_CHECK(top_logprob.has_value() == top_token.has_value(),
-              "fdl.token_logprobs: top_logprob and top_token go together");
-  auto f32 = [&](const Tensor& t, int64_t n, const char* name) {
-    TORCH_CHECK(t.is_cuda() && t.device() == logits.device() && t.scalar_type() == at::kFloat && t.is_contiguous() &&
-                    t.numel() == n,
-                "fdl.token_logprobs: ", name, " must be a contiguous fp32 tensor of ", n, " entries on ",
-                logits.device());
-  };
-  f32(logprob, rows, "logprob");
-  f32(entropy, rows, "entropy");
-  int64_t top = 0;
-  if (top_logprob) {
-    TORCH_CHECK(top_logprob->dim() == 2, "fdl.token_logprobs: top_logprob must be [rows, top]");
-    top = top_logprob->size(1);
-    f32(*top_logprob, rows * top, "top_logprob");
-    check_i64(*top_token, logits, rows * top, "top_token");
-  }
+  const int code = dtype_code(logits);
+  TORCH_CHECK(top >= 0 && top <= V, "fdl.token_logprobs: top is ", top, " of ", V, " tokens");
   c10::cuda::CUDAGuard guard(logits.device());
+  auto make = [&](at::IntArrayRef size, at::ScalarType type) {
+    return at::detail::empty_cuda(size, type, logits.device(), std::nullopt);
+  };
+  Tensor logprob = make({rows}, at::kFloat), entropy = make({rows}, at::kFloat);
+  Tensor top_lp = make({rows, top}, at::kFloat), top_tok = make({rows, top}, at::kLong);
   check_rc(fdl_token_logprobs(logits.data_ptr(), rows > 1 ? logits.stride(0) : V, as_int(rows, "rows"),
-                              as_int(V, "the vocabulary"), dtype_code(logits), targets.data_ptr<int64_t>(),
+                              as_int(V, "the vocabulary"), code, targets.data_ptr<int64_t>(),
                               logprob.data_ptr<float>(), entropy.data_ptr<float>(), as_int(top, "top"),
-                              top_logprob ? top_logprob->data_ptr<float>() : nullptr,
-                              top_token ? top_token->data_ptr<int64_t>() : nullptr, cur_stream()),
+                              top ? top_lp.data_ptr<float>() : nullptr, top ? top_tok.data_ptr<int64_t>() : nullptr,
+                              cur_stream()),
            "token_logprobs");
+  return {logprob, entropy, top_lp, top_tok};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs_meta(const Tensor& logits, const Tensor&, int64_t top) {
+  const int64_t rows = logits.size(0);
+  auto f = logits.options().dtype(at::kFloat);
+  return {at::empty({rows}, f), at::empty({rows}, f), at::empty({rows, top}, f),
+          at::empty({rows, top}, logits.options().dtype(at::kLong))};
 }
 
 // Functional form with the signature of the flash_kvcache custom op of
@@ -867,8 +868,7 @@ TORCH_LIBRARY(fdl, m) {
         "bool interleaved, float rope_scale, Tensor(a!) q, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor slots) -> ()");
   m.def("paged_decode_attn(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor lens, float scale, "
         "Tensor(a!) out) -> ()");
-  m.def("token_logprobs(Tensor logits, Tensor targets, Tensor(a!) logprob, Tensor(b!) entropy, "
-        "Tensor(c!)? top_logprob, Tensor(d!)? top_token) -> ()");
+  m.def("token_logprobs(Tensor logits, Tensor targets, int top) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("add_rmsnorm(Tensor x, Tensor res, Tensor? weight, float eps, Tensor(a!)? sum_out, Tensor(b!) normed) -> ()");
 }
 
@@ -935,8 +935,7 @@ TORCH_LIBRARY_IMPL(fdl, Meta, m) {
             double, bool, double, const Tensor&, const Tensor&, const Tensor&, const Tensor&) {});
   m.impl("paged_decode_attn", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, double,
                                  const Tensor&) {});
-  m.impl("token_logprobs", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
-                              const std::optional<Tensor>&) {});
+  m.impl("token_logprobs", &token_logprobs_meta);
   m.impl("add_rmsnorm", [](const Tensor&, const Tensor&, const std::optional<Tensor>&, double,
                            const std::optional<Tensor>&, const Tensor&) {});
 }

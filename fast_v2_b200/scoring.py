@@ -39,13 +39,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0) ->
         raise ValueError(f"token_logprobs: logits must be [rows, vocab], got {tuple(logits.shape)}")
     if not 0 <= top <= min(MAX_TOP, logits.shape[1]):
         raise ValueError(f"token_logprobs: top={top} is outside [0, min({MAX_TOP}, vocab={logits.shape[1]})]")
-    rows = logits.shape[0]
-    scores = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
-    logprob, entropy = scores.unbind(0)
-    top_lp = top_tok = None
-    if top:
-        top_lp = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-        top_tok = torch.empty((rows, top), dtype=torch.int64, device=logits.device)
-    torch.ops.fdl.token_logprobs.default(logits, targets, logprob, entropy, top_lp, top_tok)
+    logprob, entropy, top_logprob, top_token = torch.ops.fdl.token_logprobs.default(logits, targets, top)
     _lib.count_launches(1)
-    return TokenScores(logprob, entropy, top_lp, top_tok)
+    if not top:
+        top_logprob = top_token = None
+    return TokenScores(logprob, entropy, top_logprob, top_token)
