@@ -9,35 +9,38 @@
 // NaN, +inf, or nothing above -inf) gives NaN everywhere and tokens -1, and
 // is reported.
 //
-// Bound by HBM (the special-function unit is at 70% of its rate at the copy
-// rate in a 16-bit type), so the row is read once: a cluster of 1 to 8 CTAs
-// takes a row, every thread walks 16-byte vectors of it with sums relative to
-// a reference of its own (moved only when a logit passes it by kTokSlack) and
-// remembers the largest logit it saw and where.
+// Bound by HBM (with 16-bit logits the special-function unit is at 70% of its
+// rate, and the issue slots at 50%, at the copy rate), so the row is read
+// once: a cluster of 1 to 8 CTAs takes a row, every thread walks 16-byte
+// vectors of it with sums relative to a reference of its own (moved only when
+// a logit passes it by kTokSlack) and remembers the largest logit it saw and
+// where.  The sums are kept for powers of two, 2^(x log2 e - ref'), one fused
+// multiply-add an entry; ref' is the rounded ref * log2 e, and what the
+// rounding is off is known exactly and put right at the end.
 //
 // The top k need no second pass over the row.  Order all entries by (logit,
-// lower index first).  If each of W warps has r >= k / W threads whose largest
-// entry is at or above tau, then at least k entries are, so every one of the
-// top k is -- and lies with a thread whose largest entry is at or above tau.
-// tau is the smallest over these warps of the r-th largest thread maximum;
-// only the vectors of the threads at or above it are read again (some tens of
-// the 512, from L2), the entries at or above tau are collected and sorted: in
-// each warp by a bitonic network, then list by list in a tree that keeps the
-// best 32.  Rows with very many entries above tau (long runs of equal logits,
-// say) overflow the list; the k-th best of the entries caught is then a
-// better tau.
+// lower index first).  If there are k threads whose largest entry is at or
+// above tau, then at least k entries are, so every one of the top k is -- and
+// lies with a thread whose largest entry is at or above tau.  tau is the k-th
+// largest of the r = ceil(k / W) largest thread maxima of each of W warps;
+// only the vectors of the threads at or above it are read again (k and a few,
+// from L2), the entries at or above tau are collected and ranked by counting.
+// Rows with very many entries above tau (long runs of equal logits, say)
+// overflow the list; the k-th best of the entries caught is then a better tau.
 #pragma once
 #include "common.cuh"
 #include "device_util.cuh"
+#include "sm100_ptx.cuh"
 
 namespace fdl {
 
 constexpr int kTokThreads = 512;
 constexpr int kTokWarps = kTokThreads / 32;
 constexpr int kTokMaxTop = 32;
-constexpr int kTokUnroll = 4;     // vectors in flight a thread
+constexpr int kTokUnroll = 4;  // vectors in flight a thread
 constexpr float kTokSlack = 10.f;
 constexpr float kTokLog2e = 1.4426950408889634f;
+constexpr float kTokBig = 1048576.f;  // 2^20: its product with log2 e rounds by 2^-4 at most
 constexpr float kTokFloor = -1000.f;  // exp() of it is 0 in fp32; keeps 0 * inf out of t
 
 struct TokScoreArgs {
@@ -79,24 +82,24 @@ __device__ __forceinline__ uint64_t warp_sort(uint64_t key) {
     for (int off = size / 2; off > 0; off >>= 1) key = exchange(key, off, (threadIdx.x & size & 31) == 0);
   return key;
 }
-// The best 32 of two sorted lists, sorted: lane i holds one, and is given
-// entry 31 - i of the other.
-__device__ __forceinline__ uint64_t warp_merge(uint64_t key, uint64_t other_reversed) {
-  key = max64(key, other_reversed);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) key = exchange(key, off, true);
-  return key;
-}
-// Warps 0 .. lists - 1 hold a sorted list each; warp 0 ends with the best 32.
-// Every thread of the CTA calls it; sh is free again after the next barrier.
-__device__ __forceinline__ uint64_t block_merge(uint64_t key, int lists, uint64_t (*sh)[32]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int step = 1; step < lists; step <<= 1) {
-    if (warp < lists && (warp & (2 * step - 1)) == step) sh[warp][lane] = key;
-    __syncthreads();
-    if ((warp & (2 * step - 1)) == 0 && warp + step < lists) key = warp_merge(key, sh[warp + step][31 - lane]);
+// The CTA ranks the n <= kTokThreads keys of `cand` (distinct; an odd n is
+// padded with a zero) by counting the larger ones, 4, 2 or 1 threads a
+// key, and puts the best 32 in order.
+__device__ __forceinline__ void block_rank(const uint64_t* cand, int n, uint64_t* best) {
+  const int q = n * 4 <= kTokThreads ? 4 : n * 2 <= kTokThreads ? 2 : 1;
+  const int i = threadIdx.x / q, part = threadIdx.x % q;
+  const uint64_t key = i < n ? cand[i] : 0;
+  int above = 0;
+  if (i < n) {
+    const ulonglong2* c = reinterpret_cast<const ulonglong2*>(cand);
+    for (int j = part; j < (n + 1) / 2; j += q) {
+      const ulonglong2 o = c[j];
+      above += (o.x > key) + (o.y > key);
+    }
   }
-  return key;
+  if (q >= 2) above += __shfl_xor_sync(0xffffffffu, above, 1);
+  if (q == 4) above += __shfl_xor_sync(0xffffffffu, above, 2);
+  if (i < n && part == 0 && above < kTokMaxTop) best[above] = key;
 }
 
 template <typename T>
@@ -114,14 +117,15 @@ struct TokVec {  // 16 bytes of logits
     }
   }
   __device__ __forceinline__ float max() const {
-    float m = f[0];
+    float m = fmaxf(f[0], f[1]);
 #pragma unroll
-    for (int e = 1; e < kN; ++e) m = fmaxf(m, f[e]);
+    for (int e = 2; e < kN; e += 2) m = ptx::fmax3(m, f[e], f[e + 1]);
     return m;
   }
 };
 
-// Sums relative to a reference: z = sum exp(x - ref), t = sum exp(x - ref) (x - ref).
+// Sums relative to a reference: z = sum exp(x - ref), t = sum exp(x - ref) (x
+// - ref).
 struct TokSums {
   float ref, z, t;
   __device__ __forceinline__ void move(float to) {  // to >= ref
@@ -139,14 +143,53 @@ struct TokSums {
   }
 };
 
+// The same with powers of two, two entries at a time: y = x log2 e - refl, z =
+// sum 2^y, t = sum 2^y y.  The reference starts at -kTokBig, below which every
+// entry counts as 0; a row whose largest entry is outside +-kTokBig is summed
+// again with TokSums.
+struct TokSums2 {
+  float ref, refl;
+  uint64_t z, t;
+  __device__ __forceinline__ void start() {
+    ref = -kTokBig;
+    refl = ref * kTokLog2e;
+    z = t = 0;
+  }
+  __device__ __forceinline__ void move(float to) {
+    const float l = to * kTokLog2e, d = fmaxf(refl - l, 2.f * kTokFloor), f = ex2(d);
+    const uint64_t f2 = ptx::pack2(f, f);
+    t = ptx::mul2(f2, ptx::fma2(ptx::pack2(d, d), z, t));
+    z = ptx::mul2(f2, z);
+    ref = to;
+    refl = l;
+  }
+  __device__ __forceinline__ void add(float x0, float x1) {
+    float y0, y1;
+    ptx::unpack2(ptx::fma2(ptx::pack2(x0, x1), ptx::pack2(kTokLog2e, kTokLog2e), ptx::pack2(-refl, -refl)), y0, y1);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y0) : "f"(2.f * kTokFloor));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y1) : "f"(2.f * kTokFloor));
+    const uint64_t e = ptx::pack2(ex2(y0), ex2(y1));
+    z = ptx::add2(z, e);
+    t = ptx::fma2(e, ptx::pack2(y0, y1), t);
+  }
+  __device__ __forceinline__ TokSums natural() const {
+    float z0, z1, t0, t1;
+    ptx::unpack2(z, z0, z1);
+    ptx::unpack2(t, t0, t1);
+    const float r = fmaf(ref, kTokLog2e, -refl);  // exact: what refl is off
+    const float zz = z0 + z1, f = ex2(-r);
+    return TokSums{ref, zz * f, f * fmaf(-r, zz, t0 + t1) * 0.6931471805599453f};
+  }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_constant__ TokScoreArgs a) {
   constexpr int kN = TokVec<T>::kN;
   __shared__ float sh_m[kTokWarps], sh_z[kTokWarps], sh_t[kTokWarps];
-  __shared__ uint64_t sh_tau[kTokWarps];
-  __shared__ uint64_t sh_list[kTokWarps][32];
-  __shared__ uint64_t sh_cand[kTokThreads];
-  __shared__ uint64_t sh_top[32];
+  __shared__ uint64_t sh_max[kTokWarps + kTokMaxTop];  // the largest thread maxima of each warp
+  __shared__ uint64_t sh_tau;
+  __shared__ __align__(16) uint64_t sh_cand[kTokThreads];
+  __shared__ uint64_t sh_top[kTokMaxTop];
   __shared__ float4 sh_sum;
   __shared__ int sh_n;
   await_stream();
@@ -169,7 +212,8 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
   if (rank == ranks - 1 && threadIdx.x >= 32 && threadIdx.x - 32 < rest) single = a.V - rest + threadIdx.x - 32;
 
   // ---- the one pass
-  TokSums s{-3.402823466e38f, 0.f, 0.f};
+  TokSums2 s2;
+  s2.start();
   float best = -INFINITY;  // largest entry in this thread's vectors, and the first vector that has it
   int at = threadIdx.x;
   auto take = [&](uint4 u, int v) {
@@ -179,9 +223,9 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
       best = m;
       at = v;
     }
-    if (m > s.ref + kTokSlack) s.move(m);
+    if (m > s2.ref + kTokSlack) s2.move(m);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) s.add(q.f[e]);
+    for (int e = 0; e < kN; e += 2) s2.add(q.f[e], q.f[e + 1]);
   };
   int v = threadIdx.x;
   for (; v + (kTokUnroll - 1) * kTokThreads < nv; v += kTokUnroll * kTokThreads) {
@@ -192,6 +236,7 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
     for (int i = 0; i < kTokUnroll; ++i) take(u[i], v + i * kTokThreads);
   }
   for (; v < nv; v += kTokThreads) take(ld_stream16(vec + static_cast<int64_t>(v) * 16), v);
+  TokSums s = s2.natural();
   float lone = -INFINITY;
   if (single >= 0) {
     lone = static_cast<float>(x[single]);
@@ -204,33 +249,47 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   if (lane == 0) sh_m[warp] = m;
-  // the r-th largest thread maximum of the warp; a maximum counts as the last
+  // the r largest thread maxima of each warp; a maximum counts as the last
   // entry of its vector, mine + kN - 1 is the first
   const uint64_t mine = threadIdx.x < nv ? score_key(best, first + at * kN + kN - 1) : 0;
   const int full = min(nv / 32, kTokWarps);  // warps with a vector for every thread
-  if (a.top > 0 && warp < full) {
-    const int r = (a.top + full - 1) / full;
-    uint64_t big = 0;
+  const int r = full > 0 ? (a.top + full - 1) / full : 0;
+  if (warp < full) {
     if (r <= 2) {
       uint64_t left = mine;
       for (int i = 0; i < r; ++i) {
-        big = left;
+        uint64_t big = left;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) big = max64(big, __shfl_xor_sync(0xffffffffu, big, off));
         if (left == big) left = 0;
+        if (lane == 0) sh_max[warp * r + i] = big;
       }
     } else {
-      big = __shfl_sync(0xffffffffu, warp_sort(mine), r - 1);
+      const uint64_t key = warp_sort(mine);
+      if (lane < r) sh_max[warp * r + lane] = key;
     }
-    if (lane == 0) sh_tau[warp] = big;
   }
-  if (threadIdx.x == 0) sh_n = 0;
+  if (threadIdx.x == 0) {
+    sh_n = 0;
+    sh_tau = 0;  // below 32 vectors all entries fit the list
+  }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kTokWarps; ++w) m = fmaxf(m, sh_m[w]);
-  // a CTA that has seen nothing above -inf keeps z = 0
-  s.move(fmaxf(m, s.ref));
-  const float ref = s.ref;  // threads without a larger entry agree on max(m, lowest)
+  if (fabsf(m) > kTokBig && m > -INFINITY) {  // sizes that powers of two with a rounded reference do not hold
+    s = TokSums{-3.402823466e38f, 0.f, 0.f};
+    if (m > s.ref) s.move(m);
+    for (int i = threadIdx.x; i < nv; i += kTokThreads) {
+      const TokVec<T> q(*reinterpret_cast<const uint4*>(vec + static_cast<int64_t>(i) * 16));
+#pragma unroll
+      for (int e = 0; e < kN; ++e) s.add(q.f[e]);
+    }
+    if (single >= 0) s.add(lone);
+  } else if (m > s.ref) {
+    s.move(m);
+  }
+  // (a CTA that has seen nothing above -inf keeps z = 0)
+  const float ref = s.ref;
   float z = s.z, t = s.t;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -241,13 +300,18 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
     sh_z[warp] = z;
     sh_t[warp] = t;
   }
+  if (threadIdx.x < full * r) {  // the k-th largest of them
+    const uint64_t key = sh_max[threadIdx.x];
+    int above = 0;
+    for (int i = 0; i < full * r; ++i) above += sh_max[i] > key;
+    if (above == a.top - 1) sh_tau = key;
+  }
+  __syncthreads();
 
   // ---- the top entries of the CTA
-  uint64_t key = 0;
   if (a.top > 0) {
-    uint64_t tau = full > 0 ? sh_tau[0] : 0;  // below 32 vectors all entries fit the list
-    for (int w = 1; w < full; ++w) tau = min64(tau, sh_tau[w]);
     for (;;) {
+      const uint64_t tau = sh_tau;
       auto offer = [&](float f, int idx) {
         const uint64_t k = score_key(f, idx);
         if (k >= tau) {
@@ -265,20 +329,20 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
       }
       if (single >= 0) offer(lone, single);
       __syncthreads();
-      const int n = sh_n;
-      // warps behind the last candidate hold empty lists
-      key = threadIdx.x < min(n, kTokThreads) ? sh_cand[threadIdx.x] : 0;
-      if (warp * 32 < n) key = warp_sort(key);
-      key = block_merge(key, (min(n, kTokThreads) + 31) / 32, sh_list);
-      if (n <= kTokThreads) break;
-      if (threadIdx.x == a.top - 1) sh_tau[0] = key;
+      const int n = sh_n, have = min(n, kTokThreads);
+      if (have % 2 && threadIdx.x == 0) sh_cand[have] = 0;
+      if (threadIdx.x < kTokMaxTop && threadIdx.x >= have) sh_top[threadIdx.x] = 0;
       __syncthreads();
-      tau = sh_tau[0];
-      if (threadIdx.x == 0) sh_n = 0;
+      block_rank(sh_cand, have, sh_top);
+      __syncthreads();
+      if (n <= kTokThreads) break;
+      if (threadIdx.x == 0) {
+        sh_tau = sh_top[a.top - 1];
+        sh_n = 0;
+      }
       __syncthreads();
     }
   }
-  __syncthreads();
   z = t = 0.f;
 #pragma unroll
   for (int w = 0; w < kTokWarps; ++w) {
@@ -287,30 +351,46 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
   }
   TokSums row_s{ref, z, t};
   if (ranks > 1) {
-    if (warp == 0) sh_top[lane] = key;
     if (threadIdx.x == 0) sh_sum = make_float4(ref, z, t, 0.f);
     cluster_sync();
     if (rank == 0) {
-      for (uint32_t r = 1; r < ranks; ++r) {
-        const float4 o = ld_cluster4(smem_addr(&sh_sum), r);
-        TokSums other{o.x, o.y, o.z};
-        const float to = fmaxf(row_s.ref, other.ref);
-        row_s.move(to);
-        other.move(to);
-        row_s.z += other.z;
-        row_s.t += other.t;
+      // every warp joins the sums, lane by lane
+      TokSums o{-3.402823466e38f, 0.f, 0.f};
+      if (lane < ranks) {
+        const float4 f = ld_cluster4(smem_addr(&sh_sum), lane);
+        o = TokSums{f.x, f.y, f.z};
       }
+      float to = o.ref;
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, off));
+      to = __shfl_sync(0xffffffffu, to, 0);
+      o.move(to);
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) {
+        o.z += __shfl_xor_sync(0xffffffffu, o.z, off);
+        o.t += __shfl_xor_sync(0xffffffffu, o.t, off);
+      }
+      row_s = TokSums{to, __shfl_sync(0xffffffffu, o.z, 0), __shfl_sync(0xffffffffu, o.t, 0)};
       if (a.top > 0) {
-        if (warp > 0 && warp < ranks) {
-          const float2 k2 = ld_cluster2(smem_addr(&sh_top[lane]), warp);
-          key = static_cast<uint64_t>(__float_as_uint(k2.y)) << 32 | __float_as_uint(k2.x);
+        const int n = static_cast<int>(ranks) * a.top;
+        if (threadIdx.x < n) {
+          const float2 k2 = ld_cluster2(smem_addr(&sh_top[threadIdx.x % a.top]), threadIdx.x / a.top);
+          // empty entries (a CTA with fewer than k entries) stay distinct
+          const uint64_t k = static_cast<uint64_t>(__float_as_uint(k2.y)) << 32 | __float_as_uint(k2.x);
+          sh_cand[threadIdx.x] = k ? k : threadIdx.x + 1;
         }
-        key = block_merge(key, ranks, sh_list);
+        if (n % 2 && threadIdx.x == 0) sh_cand[n] = 0;
+        __syncthreads();
       }
     }
-    cluster_sync();  // no CTA leaves while its shared memory is read
+    cluster_sync();  // no CTA leaves (or ranks into sh_top) while its shared memory is read
     if (rank != 0) return;
+    if (a.top > 0) {
+      block_rank(sh_cand, static_cast<int>(ranks) * a.top, sh_top);
+      __syncthreads();
+    }
   }
+  const uint64_t key = threadIdx.x < a.top ? sh_top[threadIdx.x] : 0;
   const bool bad = !(row_s.z > 0.f && row_s.z < INFINITY);
   const float lz = logf(row_s.z);
   if (threadIdx.x == 0) {
