@@ -28,16 +28,19 @@
 // Rows with very many entries above tau (long runs of equal logits, say)
 // overflow the list; the k-th best of the entries caught is then a better tau.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "device_util.cuh"
 #include "sm100_ptx.cuh"
 
 namespace fdl {
 
-constexpr int kTokThreads = 512;
+constexpr int kTokThreads = 256;
 constexpr int kTokWarps = kTokThreads / 32;
 constexpr int kTokMaxTop = 32;
-constexpr int kTokUnroll = 4;  // vectors in flight a thread
+constexpr int kTokList = 512;  // entries above tau that are caught (a cluster of 8 brings 8 * 32)
+constexpr int kTokUnroll = 2;  // vectors in flight a thread
 constexpr float kTokSlack = 10.f;
 constexpr float kTokLog2e = 1.4426950408889634f;
 constexpr float kTokBig = 1048576.f;  // 2^20: its product with log2 e rounds by 2^-4 at most
@@ -82,24 +85,40 @@ __device__ __forceinline__ uint64_t warp_sort(uint64_t key) {
     for (int off = size / 2; off > 0; off >>= 1) key = exchange(key, off, (threadIdx.x & size & 31) == 0);
   return key;
 }
-// The CTA ranks the n <= kTokThreads keys of `cand` (distinct; an odd n is
-// padded with a zero) by counting the larger ones, 4, 2 or 1 threads a
-// key, and puts the best 32 in order.
+// The CTA ranks n <= kTokList distinct keys by counting the larger ones and
+// puts the best 32 in order; four threads a key where there are enough.
 __device__ __forceinline__ void block_rank(const uint64_t* cand, int n, uint64_t* best) {
-  const int q = n * 4 <= kTokThreads ? 4 : n * 2 <= kTokThreads ? 2 : 1;
-  const int i = threadIdx.x / q, part = threadIdx.x % q;
-  const uint64_t key = i < n ? cand[i] : 0;
-  int above = 0;
-  if (i < n) {
-    const ulonglong2* c = reinterpret_cast<const ulonglong2*>(cand);
-    for (int j = part; j < (n + 1) / 2; j += q) {
-      const ulonglong2 o = c[j];
-      above += (o.x > key) + (o.y > key);
+  const int q = n * 4 <= kTokThreads ? 4 : 1, part = threadIdx.x % q;
+  for (int i0 = 0; i0 < n; i0 += kTokThreads) {
+    const int i = i0 + threadIdx.x / q;
+    const uint64_t key = i < n ? cand[i] : 0;
+    int above = 0;
+    if (i < n)
+      for (int j = part; j < n; j += q) above += cand[j] > key;
+    if (q == 4) {
+      above += __shfl_xor_sync(0xffffffffu, above, 1);
+      above += __shfl_xor_sync(0xffffffffu, above, 2);
     }
+    if (i < n && part == 0 && above < kTokMaxTop) best[above] = key;
   }
-  if (q >= 2) above += __shfl_xor_sync(0xffffffffu, above, 1);
-  if (q == 4) above += __shfl_xor_sync(0xffffffffu, above, 2);
-  if (i < n && part == 0 && above < kTokMaxTop) best[above] = key;
+}
+
+// The finite floor that -inf is raised to in the fast sums.
+template <typename T>
+constexpr float kTokLowest = std::is_same<T, __half>::value ? -65504.f : -1.2676506e30f;  // -2^100
+// max(x, floor) that keeps a NaN, for the entries in a word of logits.
+template <typename T>
+__device__ __forceinline__ uint32_t clamp_word(uint32_t u) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(u) : "r"(0xf180f180u));  // -2^100
+  else if constexpr (std::is_same<T, __half>::value)
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(u) : "r"(0xfbfffbffu));  // -65504
+  else {
+    float f = __uint_as_float(u);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(f) : "f"(kTokLowest<T>));
+    u = __float_as_uint(f);
+  }
+  return u;
 }
 
 template <typename T>
@@ -115,6 +134,11 @@ struct TokVec {  // 16 bytes of logits
     } else {
       unpack8<T>(u, f);
     }
+  }
+  // With -inf (and what is below a finite floor) raised to the floor, whose
+  // exponential is 0 next to any reference that the fast sums allow.
+  __device__ __forceinline__ static TokVec finite(uint4 u) {
+    return TokVec(make_uint4(clamp_word<T>(u.x), clamp_word<T>(u.y), clamp_word<T>(u.z), clamp_word<T>(u.w)));
   }
   __device__ __forceinline__ float max() const {
     float m = fmaxf(f[0], f[1]);
@@ -143,8 +167,8 @@ struct TokSums {
   }
 };
 
-// The same with powers of two, two entries at a time: y = x log2 e - refl, z =
-// sum 2^y, t = sum 2^y y.  The reference starts at -kTokBig, below which every
+// The same with powers of two, two finite entries at a time: y = x log2 e -
+// refl, z = sum 2^y, t = sum 2^y y.  The reference starts at -kTokBig, below which every
 // entry counts as 0; a row whose largest entry is outside +-kTokBig is summed
 // again with TokSums.
 struct TokSums2 {
@@ -165,12 +189,11 @@ struct TokSums2 {
   }
   __device__ __forceinline__ void add(float x0, float x1) {
     float y0, y1;
-    ptx::unpack2(ptx::fma2(ptx::pack2(x0, x1), ptx::pack2(kTokLog2e, kTokLog2e), ptx::pack2(-refl, -refl)), y0, y1);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y0) : "f"(2.f * kTokFloor));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y1) : "f"(2.f * kTokFloor));
+    const uint64_t y = ptx::fma2(ptx::pack2(x0, x1), ptx::pack2(kTokLog2e, kTokLog2e), ptx::pack2(-refl, -refl));
+    ptx::unpack2(y, y0, y1);
     const uint64_t e = ptx::pack2(ex2(y0), ex2(y1));
     z = ptx::add2(z, e);
-    t = ptx::fma2(e, ptx::pack2(y0, y1), t);
+    t = ptx::fma2(e, y, t);
   }
   __device__ __forceinline__ TokSums natural() const {
     float z0, z1, t0, t1;
@@ -183,12 +206,12 @@ struct TokSums2 {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_constant__ TokScoreArgs a) {
+__global__ void __launch_bounds__(kTokThreads, 4) token_scores_kernel(const __grid_constant__ TokScoreArgs a) {
   constexpr int kN = TokVec<T>::kN;
   __shared__ float sh_m[kTokWarps], sh_z[kTokWarps], sh_t[kTokWarps];
   __shared__ uint64_t sh_max[kTokWarps + kTokMaxTop];  // the largest thread maxima of each warp
   __shared__ uint64_t sh_tau;
-  __shared__ __align__(16) uint64_t sh_cand[kTokThreads];
+  __shared__ __align__(16) uint64_t sh_cand[kTokList];
   __shared__ uint64_t sh_top[kTokMaxTop];
   __shared__ float4 sh_sum;
   __shared__ int sh_n;
@@ -214,28 +237,46 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
   // ---- the one pass
   TokSums2 s2;
   s2.start();
-  float best = -INFINITY;  // largest entry in this thread's vectors, and the first vector that has it
+  // largest entry in this thread's vectors, the first vector that has it, and
+  // the largest entry of the others
+  float best = -INFINITY, second = -INFINITY;
   int at = threadIdx.x;
   auto take = [&](uint4 u, int v) {
-    const TokVec<T> q(u);
+    const TokVec<T> q = TokVec<T>::finite(u);
     const float m = q.max();
-    if (m > best) {
-      best = m;
-      at = v;
-    }
+    second = fmaxf(second, fminf(m, best));
+    if (m > best) at = v;
+    best = fmaxf(m, best);
     if (m > s2.ref + kTokSlack) s2.move(m);
 #pragma unroll
     for (int e = 0; e < kN; e += 2) s2.add(q.f[e], q.f[e + 1]);
   };
-  int v = threadIdx.x;
-  for (; v + (kTokUnroll - 1) * kTokThreads < nv; v += kTokUnroll * kTokThreads) {
-    uint4 u[kTokUnroll];
+  {
+    // the next batch is on its way while one is summed
+    auto fetch = [&](uint4 (&u)[kTokUnroll], int v) {
 #pragma unroll
-    for (int i = 0; i < kTokUnroll; ++i) u[i] = ld_stream16(vec + static_cast<int64_t>(v + i * kTokThreads) * 16);
+      for (int i = 0; i < kTokUnroll; ++i)
+        if (v + i * kTokThreads < nv) u[i] = ld_stream16(vec + static_cast<int64_t>(v + i * kTokThreads) * 16);
+    };
+    auto sum = [&](const uint4 (&u)[kTokUnroll], int v) {
 #pragma unroll
-    for (int i = 0; i < kTokUnroll; ++i) take(u[i], v + i * kTokThreads);
+      for (int i = 0; i < kTokUnroll; ++i)
+        if (v + i * kTokThreads < nv) take(u[i], v + i * kTokThreads);
+    };
+    uint4 a0[kTokUnroll], a1[kTokUnroll];
+    constexpr int kBatch = kTokUnroll * kTokThreads;
+    int v = threadIdx.x;
+    fetch(a0, v);
+    while (v < nv) {
+      fetch(a1, v + kBatch);
+      sum(a0, v);
+      v += kBatch;
+      if (v >= nv) break;
+      fetch(a0, v + kBatch);
+      sum(a1, v);
+      v += kBatch;
+    }
   }
-  for (; v < nv; v += kTokThreads) take(ld_stream16(vec + static_cast<int64_t>(v) * 16), v);
   TokSums s = s2.natural();
   float lone = -INFINITY;
   if (single >= 0) {
@@ -249,9 +290,13 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   if (lane == 0) sh_m[warp] = m;
-  // the r largest thread maxima of each warp; a maximum counts as the last
-  // entry of its vector, mine + kN - 1 is the first
-  const uint64_t mine = threadIdx.x < nv ? score_key(best, first + at * kN + kN - 1) : 0;
+  // The r largest thread maxima of each warp.  A thread's largest entry is
+  // between mine (the last entry of its vector; -inf where the floor hides
+  // it) and mine_most (the first one).
+  const bool hidden = !(best > kTokLowest<T>);
+  const uint64_t mine =
+      threadIdx.x < nv ? score_key(hidden ? -INFINITY : best, first + at * kN + kN - 1) : 0;
+  const uint64_t mine_most = hidden ? score_key(best, 0) : mine + (kN - 1);
   const int full = min(nv / 32, kTokWarps);  // warps with a vector for every thread
   const int r = full > 0 ? (a.top + full - 1) / full : 0;
   if (warp < full) {
@@ -273,22 +318,35 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
     sh_n = 0;
     sh_tau = 0;  // below 32 vectors all entries fit the list
   }
+  if (threadIdx.x < kTokMaxTop) sh_top[threadIdx.x] = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kTokWarps; ++w) m = fmaxf(m, sh_m[w]);
-  if (fabsf(m) > kTokBig && m > -INFINITY) {  // sizes that powers of two with a rounded reference do not hold
-    s = TokSums{-3.402823466e38f, 0.f, 0.f};
-    if (m > s.ref) s.move(m);
-    for (int i = threadIdx.x; i < nv; i += kTokThreads) {
-      const TokVec<T> q(*reinterpret_cast<const uint4*>(vec + static_cast<int64_t>(i) * 16));
+  if (fabsf(m) > kTokBig || m <= kTokLowest<T>) {
+    // Sizes that the fast sums do not hold: again, with the true maximum.  (A
+    // CTA that sees nothing above -inf keeps z = 0.)
+    auto each = [&](auto f) {
+      for (int i = threadIdx.x; i < nv; i += kTokThreads) {
+        const TokVec<T> q(*reinterpret_cast<const uint4*>(vec + static_cast<int64_t>(i) * 16));
 #pragma unroll
-      for (int e = 0; e < kN; ++e) s.add(q.f[e]);
-    }
-    if (single >= 0) s.add(lone);
+        for (int e = 0; e < kN; ++e) f(q.f[e]);
+      }
+      if (single >= 0) f(lone);
+    };
+    m = -INFINITY;
+    each([&](float x) { m = fmaxf(m, x); });
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    __syncthreads();
+    if (lane == 0) sh_m[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kTokWarps; ++w) m = fmaxf(m, sh_m[w]);
+    s = TokSums{fmaxf(m, -3.402823466e38f), 0.f, 0.f};
+    each([&](float x) { s.add(x); });
   } else if (m > s.ref) {
     s.move(m);
   }
-  // (a CTA that has seen nothing above -inf keeps z = 0)
   const float ref = s.ref;
   float z = s.z, t = s.t;
 #pragma unroll
@@ -316,26 +374,26 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
         const uint64_t k = score_key(f, idx);
         if (k >= tau) {
           const int n = atomicAdd(&sh_n, 1);
-          if (n < kTokThreads) sh_cand[n] = k;
+          if (n < kTokList) sh_cand[n] = k;
         }
       };
-      for (unsigned who = __ballot_sync(0xffffffffu, threadIdx.x < nv && mine + (kN - 1) >= tau); who; who &= who - 1) {
-        const int owner = warp * 32 + __ffs(who) - 1;
-        for (int i = owner + lane * kTokThreads; i < nv; i += 32 * kTokThreads) {
-          const TokVec<T> q(*reinterpret_cast<const uint4*>(vec + static_cast<int64_t>(i) * 16));
+      auto offer_vector = [&](int i) {
+        const TokVec<T> q(*reinterpret_cast<const uint4*>(vec + static_cast<int64_t>(i) * 16));
 #pragma unroll
-          for (int e = 0; e < kN; ++e) offer(q.f[e], first + i * kN + e);
-        }
-      }
+        for (int e = 0; e < kN; ++e) offer(q.f[e], first + i * kN + e);
+      };
+      const bool in = threadIdx.x < nv && mine_most >= tau;
+      const bool more = in && (hidden || score_key(second, 0) >= tau);  // other vectors may have one
+      if (in && !more) offer_vector(at);
       if (single >= 0) offer(lone, single);
+      // the warp reads all vectors of such a thread
+      for (unsigned who = __ballot_sync(0xffffffffu, more); who; who &= who - 1)
+        for (int i = warp * 32 + __ffs(who) - 1 + lane * kTokThreads; i < nv; i += 32 * kTokThreads) offer_vector(i);
       __syncthreads();
-      const int n = sh_n, have = min(n, kTokThreads);
-      if (have % 2 && threadIdx.x == 0) sh_cand[have] = 0;
-      if (threadIdx.x < kTokMaxTop && threadIdx.x >= have) sh_top[threadIdx.x] = 0;
+      const int n = sh_n;
+      block_rank(sh_cand, min(n, kTokList), sh_top);
       __syncthreads();
-      block_rank(sh_cand, have, sh_top);
-      __syncthreads();
-      if (n <= kTokThreads) break;
+      if (n <= kTokList) break;
       if (threadIdx.x == 0) {
         sh_tau = sh_top[a.top - 1];
         sh_n = 0;
@@ -379,7 +437,6 @@ __global__ void __launch_bounds__(kTokThreads) token_scores_kernel(const __grid_
           const uint64_t k = static_cast<uint64_t>(__float_as_uint(k2.y)) << 32 | __float_as_uint(k2.x);
           sh_cand[threadIdx.x] = k ? k : threadIdx.x + 1;
         }
-        if (n % 2 && threadIdx.x == 0) sh_cand[n] = 0;
         __syncthreads();
       }
     }
