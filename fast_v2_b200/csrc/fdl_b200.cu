@@ -939,7 +939,7 @@ int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int voc
   // CTAs a row: enough to fill the GPU (three a SM) with few rows, each with
   // at least one vector a thread.
   const int64_t vectors = static_cast<int64_t>(vocab) * (dtype == FDL_F32 ? 4 : 2) / 16;
-  static const int env_t = getenv("FDL_T") ? atoi(getenv("FDL_T")) : 5;
+  static const int env_t = getenv("FDL_T") ? atoi(getenv("FDL_T")) : 2;
   int cluster = 1;
   while (cluster < 8 && static_cast<int64_t>(rows) * cluster < static_cast<int64_t>(env_t) * num_sms() && vectors >= 2ll * cluster * kTokThreads)
     cluster *= 2;

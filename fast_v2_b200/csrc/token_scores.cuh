@@ -40,7 +40,7 @@ constexpr int kTokThreads = 256;
 constexpr int kTokWarps = kTokThreads / 32;
 constexpr int kTokMaxTop = 32;
 constexpr int kTokList = 512;  // entries above tau that are caught (a cluster of 8 brings 8 * 32)
-constexpr int kTokUnroll = 2;  // vectors in flight a thread
+constexpr int kTokUnroll = 3;  // vectors in flight a thread
 constexpr float kTokSlack = 10.f;
 constexpr float kTokLog2e = 1.4426950408889634f;
 constexpr float kTokBig = 1048576.f;  // 2^20: its product with log2 e rounds by 2^-4 at most
@@ -234,47 +234,69 @@ __global__ void __launch_bounds__(kTokThreads, 4) token_scores_kernel(const __gr
   if (rank == 0 && threadIdx.x < head) single = threadIdx.x;
   if (rank == ranks - 1 && threadIdx.x >= 32 && threadIdx.x - 32 < rest) single = a.V - rest + threadIdx.x - 32;
 
-  // ---- the one pass
+  // the target's logit is on its way from the start
+  int64_t target = -1;
+  float target_x = 0.f;
+  if (rank == 0 && threadIdx.x == 0) {
+    target = a.targets[row];
+    if (target >= 0 && target < a.V) target_x = static_cast<float>(x[target]);
+  }
+
+  // ---- the one pass, in batches of kTokUnroll vectors a thread (and the rest
+  // vector by vector)
+  constexpr int kBatch = kTokUnroll * kTokThreads;
+  const int whole = nv / kBatch * kBatch;
   TokSums2 s2;
   s2.start();
-  // largest entry in this thread's vectors, the first vector that has it, and
-  // the largest entry of the others
+  // largest entry of this thread's batches, the first batch that has it (its
+  // first vector), and the largest entry of the others
   float best = -INFINITY, second = -INFINITY;
   int at = threadIdx.x;
-  auto take = [&](uint4 u, int v) {
-    const TokVec<T> q = TokVec<T>::finite(u);
-    const float m = q.max();
+  auto note = [&](float m, int v) {
     second = fmaxf(second, fminf(m, best));
     if (m > best) at = v;
     best = fmaxf(m, best);
     if (m > s2.ref + kTokSlack) s2.move(m);
+  };
+  auto sum = [&](const TokVec<T>& q) {
 #pragma unroll
     for (int e = 0; e < kN; e += 2) s2.add(q.f[e], q.f[e + 1]);
   };
   {
-    // the next batch is on its way while one is summed
-    auto fetch = [&](uint4 (&u)[kTokUnroll], int v) {
+    const char* p = vec + threadIdx.x * 16;
+    uint4 next[kTokUnroll];  // the next batch is on its way while one is summed
+    auto fetch = [&](int v) {
+      if (v < whole) {
 #pragma unroll
-      for (int i = 0; i < kTokUnroll; ++i)
-        if (v + i * kTokThreads < nv) u[i] = ld_stream16(vec + static_cast<int64_t>(v + i * kTokThreads) * 16);
-    };
-    auto sum = [&](const uint4 (&u)[kTokUnroll], int v) {
+        for (int i = 0; i < kTokUnroll; ++i) next[i] = ld_stream16(p + i * kTokThreads * 16);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kTokUnroll; ++i)
-        if (v + i * kTokThreads < nv) take(u[i], v + i * kTokThreads);
+        for (int i = 0; i < kTokUnroll; ++i)
+          if (v + static_cast<int>(threadIdx.x) + i * kTokThreads < nv) next[i] = ld_stream16(p + i * kTokThreads * 16);
+      }
+      p += kBatch * 16;
     };
-    uint4 a0[kTokUnroll], a1[kTokUnroll];
-    constexpr int kBatch = kTokUnroll * kTokThreads;
-    int v = threadIdx.x;
-    fetch(a0, v);
-    while (v < nv) {
-      fetch(a1, v + kBatch);
-      sum(a0, v);
-      v += kBatch;
-      if (v >= nv) break;
-      fetch(a0, v + kBatch);
-      sum(a1, v);
-      v += kBatch;
+    fetch(0);
+    for (int v = 0; v < whole; v += kBatch) {
+      uint4 u[kTokUnroll];
+#pragma unroll
+      for (int i = 0; i < kTokUnroll; ++i) u[i] = next[i];
+      fetch(v + kBatch);
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kTokUnroll; ++i) m = fmaxf(m, TokVec<T>::finite(u[i]).max());
+      note(m, v + threadIdx.x);
+#pragma unroll
+      for (int i = 0; i < kTokUnroll; ++i) sum(TokVec<T>::finite(u[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < kTokUnroll; ++i) {
+      const int v = whole + static_cast<int>(threadIdx.x) + i * kTokThreads;
+      if (v < nv) {
+        const TokVec<T> q = TokVec<T>::finite(next[i]);
+        note(q.max(), v);
+        sum(q);
+      }
     }
   }
   TokSums s = s2.natural();
@@ -291,12 +313,13 @@ __global__ void __launch_bounds__(kTokThreads, 4) token_scores_kernel(const __gr
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   if (lane == 0) sh_m[warp] = m;
   // The r largest thread maxima of each warp.  A thread's largest entry is
-  // between mine (the last entry of its vector; -inf where the floor hides
-  // it) and mine_most (the first one).
+  // between mine (the last entry of its batch; -inf where the floor hides it)
+  // and mine_most (the first one).
   const bool hidden = !(best > kTokLowest<T>);
+  const int last = at < whole ? at + (kTokUnroll - 1) * kTokThreads : at;
   const uint64_t mine =
-      threadIdx.x < nv ? score_key(hidden ? -INFINITY : best, first + at * kN + kN - 1) : 0;
-  const uint64_t mine_most = hidden ? score_key(best, 0) : mine + (kN - 1);
+      threadIdx.x < nv ? score_key(hidden ? -INFINITY : best, first + last * kN + kN - 1) : 0;
+  const uint64_t mine_most = score_key(best, hidden ? 0 : first + at * kN);
   const int full = min(nv / 32, kTokWarps);  // warps with a vector for every thread
   const int r = full > 0 ? (a.top + full - 1) / full : 0;
   if (warp < full) {
@@ -383,8 +406,9 @@ __global__ void __launch_bounds__(kTokThreads, 4) token_scores_kernel(const __gr
         for (int e = 0; e < kN; ++e) offer(q.f[e], first + i * kN + e);
       };
       const bool in = threadIdx.x < nv && mine_most >= tau;
-      const bool more = in && (hidden || score_key(second, 0) >= tau);  // other vectors may have one
-      if (in && !more) offer_vector(at);
+      const bool more = in && (hidden || score_key(second, 0) >= tau);  // other batches may have one
+      if (in && !more)
+        for (int i = at; i <= last; i += kTokThreads) offer_vector(i);
       if (single >= 0) offer(lone, single);
       // the warp reads all vectors of such a thread
       for (unsigned who = __ballot_sync(0xffffffffu, more); who; who &= who - 1)
@@ -451,15 +475,14 @@ __global__ void __launch_bounds__(kTokThreads, 4) token_scores_kernel(const __gr
   const bool bad = !(row_s.z > 0.f && row_s.z < INFINITY);
   const float lz = logf(row_s.z);
   if (threadIdx.x == 0) {
-    const int64_t tg = a.targets[row];
     float lp = 0.f;
     if (bad) {
       report(FDL_DEV_INDEX, row);
-    } else if (tg >= a.V) {
-      report(FDL_DEV_INDEX, tg);
+    } else if (target >= a.V) {
+      report(FDL_DEV_INDEX, target);
       lp = NAN;
-    } else if (tg >= 0) {
-      lp = static_cast<float>(x[tg]) - row_s.ref - lz;
+    } else if (target >= 0) {
+      lp = target_x - row_s.ref - lz;
     }
     a.logprob[row] = bad ? NAN : lp;
     a.entropy[row] = bad ? NAN : lz - row_s.t / row_s.z;
