@@ -823,15 +823,20 @@ int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos, const f
     if ((st * 2) % 16) return FDL_E_ALIGN;
   NormRopeArgs a{y, y_rs, pos, inv_freq, q_weight, k_weight, q, static_cast<char*>(k_pages),
                  static_cast<char*>(v_pages), kv_sp * 2, kv_ss * 2, kv_sh * 2, slots,
-                 static_cast<int64_t>(num_pages) * page_size, {}, eps, rope_scale, static_cast<int>(rows), hq, hkv,
-                 head_dim, 2 * n_freq};
+                 static_cast<int64_t>(num_pages) * page_size, {}, {}, {}, eps, rope_scale, static_cast<int>(rows), hq,
+                 hkv, head_dim, 2 * n_freq, 1};
   a.page.init(static_cast<uint32_t>(page_size));
+  a.heads.init(static_cast<uint32_t>(hq + 2 * hkv));
+  a.pairs.init(static_cast<uint32_t>(std::max(1, n_freq)));
   int gs = 1;
   while (gs * 16 < head_dim) gs *= 2;
-  const int64_t lanes = (static_cast<int64_t>(hq) + 2 * static_cast<int64_t>(hkv)) * gs;
-  const int threads = static_cast<int>(std::min<int64_t>(kNrMaxThreads, (lanes + 31) / 32 * 32));
+  static const int env_r = getenv("FDL_R") ? atoi(getenv("FDL_R")) : 8;
+  while (a.per < env_r && rows > static_cast<int64_t>(a.per) * 4 * num_sms()) a.per *= 2;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) { return launch_after(kernel, static_cast<unsigned>(rows), threads, 0, s, 1, a); };
+  auto go = [&](auto kernel) {
+    return launch_after(kernel, static_cast<unsigned>((rows + a.per - 1) / a.per), kNrThreads, a.per * n_freq * 8, s, 1,
+                        a);
+  };
   auto by_gs = [&](auto t, auto inter) {
     using T = decltype(t);
     constexpr bool kInter = decltype(inter)::value;

@@ -12,19 +12,22 @@
 // 2^-4 of a radian), so p * inv_freq is formed and reduced to a fraction of a
 // turn in fp64 -- three operations per pair and row, shared by all heads.
 //
-// Bound by HBM: each element is read once and written once.  A CTA holds one
-// row; a head takes GS lanes (D / 16 rounded up to a power of two), each with
-// two 16-byte vectors, so that both elements of a pair sit in one thread in
-// either layout and the norm is a shuffle over the head's lanes.  Both loads
-// are in flight before the row's cos / sin table is computed.
+// Bound by HBM: each element is read once and written once.  A CTA takes a few
+// rows (one where rows are few); a head takes GS lanes (D / 16 rounded up to a
+// power of two), each with two 16-byte vectors, so that both elements of a
+// pair sit in one thread in either layout and the norm is a shuffle over the
+// head's lanes.  The cos / sin tables of all the CTA's rows are computed in
+// one go, one pair a thread, while the first vectors are on their way, and the
+// next head's vectors are loaded while one is turned.
 #pragma once
 #include "common.cuh"
 #include "device_util.cuh"
 
 namespace fdl {
 
-constexpr int kNrMaxThreads = 512;
+constexpr int kNrThreads = 256;
 constexpr int kNrMaxDim = 256;
+constexpr int kNrMaxRows = 8;  // rows a CTA
 
 struct NormRopeArgs {
   const void* y;
@@ -40,23 +43,25 @@ struct NormRopeArgs {
   const int64_t* slots;
   int64_t n_slots;
   FastDiv page;
+  FastDiv heads;  // hq + 2 hkv
+  FastDiv pairs;  // rot / 2
   float eps, scale;
   int rows, hq, hkv, D, rot;
+  int per;  // rows a CTA
 };
 
 template <typename T, int GS, bool INTER>
-__global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
-  // (cos, sin) of pair j, ordered so that the lanes of a head read
-  // consecutive 16-byte pieces.
-  __shared__ float4 s_cs[kNrMaxDim / 4];
+__global__ void __launch_bounds__(kNrThreads, 4) norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
+  // (cos, sin) of pair j of each row, ordered so that the lanes of a head
+  // read consecutive 16-byte pieces.
+  extern __shared__ float4 s_cs[];
+  __shared__ int64_t s_at[kNrMaxRows];  // byte offset of the row's slot, or -1
   await_stream();
   release_stream();
-  const int row = blockIdx.x;
+  const int row0 = blockIdx.x * a.per, nrows = min(a.per, a.rows - row0);
   const int L = a.D / 16;        // lanes that hold elements of a head
   const int RL = a.rot / 16;     // of these, lanes that turn pairs (half layout)
-  const int heads = a.hq + 2 * a.hkv;
   const int lane = threadIdx.x % GS;
-  const char* yr = static_cast<const char*>(a.y) + static_cast<int64_t>(row) * a.y_rs * 2;
   // The two 16-byte vectors of this lane.
   int v0, v1;
   if (INTER) {
@@ -70,39 +75,53 @@ __global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_c
     v1 = 2 * lane + 1;
   }
   const bool mine = lane < L;
-  uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-  int h = threadIdx.x / GS;
-  const int hstep = blockDim.x / GS;
-  if (mine && h < heads) {
-    u0 = ld_stream16(yr + (h * a.D + v0 * 8) * 2);
-    u1 = ld_stream16(yr + (h * a.D + v1 * 8) * 2);
-  }
-  const int64_t slot = a.slots[row];
-  {
-    const double p = static_cast<double>(a.pos[row]);
-    float2* cs = reinterpret_cast<float2*>(s_cs);
-    for (int j = threadIdx.x; j < a.rot / 2; j += blockDim.x) {
-      double t = p * static_cast<double>(a.inv_freq[j]) * 0.15915494309189535;  // turns
-      t -= rint(t);
-      float sn, c;
-      sincospif(2.f * static_cast<float>(t), &sn, &c);
-      // half layout: piece i = (j % 8) / 2 of lane j / 8; interleaved: piece
-      // (j % 4) / 2 of vector j / 4
-      const int at = INTER ? ((j % 4) / 2 * (a.rot / 8) + j / 4) * 2 + j % 2 : ((j % 8) / 2 * RL + j / 8) * 2 + j % 2;
-      cs[at] = make_float2(c * a.scale, sn * a.scale);
+  const int items = nrows * static_cast<int>(a.heads.d);
+  const char* y0 = static_cast<const char*>(a.y) + static_cast<int64_t>(row0) * a.y_rs * 2;
+  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0;  // the next item's vectors
+  auto fetch = [&](int i) {
+    if (mine && i < items) {
+      uint32_t r, h;
+      a.heads.divmod(i, r, h);
+      const char* p = y0 + static_cast<int64_t>(r) * a.y_rs * 2 + h * a.D * 2;
+      n0 = ld_stream16(p + v0 * 16);
+      n1 = ld_stream16(p + v1 * 16);
     }
+  };
+  int item = threadIdx.x / GS;
+  constexpr int kStep = kNrThreads / GS;
+  fetch(item);
+  if (threadIdx.x < nrows) {
+    const int64_t slot = a.slots[row0 + threadIdx.x];
+    int64_t at = -1;
+    if (slot >= 0 && slot < a.n_slots) {
+      uint32_t page, off;  // the host refuses pools of 2^31 slots
+      a.page.divmod(static_cast<uint32_t>(slot), page, off);
+      at = static_cast<int64_t>(page) * a.sp + static_cast<int64_t>(off) * a.ss;
+    } else if (slot != -1) {
+      report(FDL_DEV_INDEX, slot);
+    }
+    s_at[threadIdx.x] = at;
   }
-  const bool store = slot >= 0 && slot < a.n_slots;
-  if (!store && slot != -1 && threadIdx.x == 0) report(FDL_DEV_INDEX, slot);
-  uint32_t pg = 0, po = 0;
-  if (store) {
-    // slots below 2^31 divide fast; the host refuses larger pools
-    a.page.divmod(static_cast<uint32_t>(slot), pg, po);
+  for (int i = threadIdx.x; i < nrows * (a.rot / 2); i += kNrThreads) {
+    uint32_t r, j;
+    a.pairs.divmod(i, r, j);
+    double t = static_cast<double>(a.pos[row0 + r]) * static_cast<double>(a.inv_freq[j]) * 0.15915494309189535;  // turns
+    t -= rint(t);
+    float sn, c;
+    sincospif(2.f * static_cast<float>(t), &sn, &c);
+    // half layout: piece (j % 8) / 2 of lane j / 8; interleaved: piece (j %
+    // 4) / 2 of vector j / 4
+    const int at = INTER ? ((j % 4) / 2 * (a.rot / 8) + j / 4) * 2 + j % 2 : ((j % 8) / 2 * RL + j / 8) * 2 + j % 2;
+    reinterpret_cast<float2*>(s_cs)[r * (a.rot / 2) + at] = make_float2(c * a.scale, sn * a.scale);
   }
-  const int64_t kv_at = static_cast<int64_t>(pg) * a.sp + static_cast<int64_t>(po) * a.ss;
   __syncthreads();
-  for (; h - static_cast<int>(threadIdx.x / GS) < heads; h += hstep) {  // every lane of a warp runs the same trips
-    const bool on = mine && h < heads;
+  for (int base = 0; base < items; base += kStep, item += kStep) {  // every lane runs the same trips
+    const uint4 u0 = n0, u1 = n1;
+    fetch(item + kStep);
+    uint32_t r, hh;
+    a.heads.divmod(min(item, items - 1), r, hh);
+    const int h = hh;
+    const bool on = mine && item < items;
     const void* w = h < a.hq ? a.qw : h < a.hq + a.hkv ? a.kw : nullptr;
     float x0[8], x1[8];
     unpack8<T>(u0, x0);
@@ -128,7 +147,9 @@ __global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_c
       }
     }
     if (on) {
-      if (h < a.hq + a.hkv) {
+      const bool copied = h >= a.hq + a.hkv;  // V keeps its bits (a NaN's payload too)
+      if (!copied) {
+        const float4* cs = s_cs + r * (a.rot / 4);
         if (INTER) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -137,7 +158,7 @@ __global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_c
             if (vv < a.rot / 8) {
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const float4 c = s_cs[i * (a.rot / 8) + vv];
+                const float4 c = cs[i * (a.rot / 8) + vv];
                 const float a0 = x[4 * i], b0 = x[4 * i + 1], a1 = x[4 * i + 2], b1 = x[4 * i + 3];
                 x[4 * i] = a0 * c.x - b0 * c.y;
                 x[4 * i + 1] = b0 * c.x + a0 * c.y;
@@ -149,7 +170,7 @@ __global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_c
         } else if (lane < RL) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float4 c = s_cs[i * RL + lane];
+            const float4 c = cs[i * RL + lane];
             const float a0 = x0[2 * i], b0 = x1[2 * i], a1 = x0[2 * i + 1], b1 = x1[2 * i + 1];
             x0[2 * i] = a0 * c.x - b0 * c.y;
             x1[2 * i] = b0 * c.x + a0 * c.y;
@@ -161,23 +182,17 @@ __global__ void __launch_bounds__(kNrMaxThreads) norm_rope_kernel(const __grid_c
       char* dst;
       bool write = true;
       if (h < a.hq) {
-        dst = static_cast<char*>(a.q) + (static_cast<int64_t>(row) * a.hq + h) * a.D * 2;
+        dst = static_cast<char*>(a.q) + ((static_cast<int64_t>(row0) + r) * a.hq + h) * a.D * 2;
       } else {
         const int kh = h - a.hq;
-        dst = kh < a.hkv ? a.k + kv_at + kh * a.sh : a.v + kv_at + (kh - a.hkv) * a.sh;
-        write = store;
+        const int64_t at = s_at[r];
+        dst = kh < a.hkv ? a.k + at + kh * a.sh : a.v + at + (kh - a.hkv) * a.sh;
+        write = at >= 0;
       }
       if (write) {
-        // heads that are only copied keep their bits (a NaN's payload too)
-        const bool same = h >= a.hq + a.hkv;
-        *reinterpret_cast<uint4*>(dst + v0 * 16) = same ? u0 : pack8<T>(x0);
-        *reinterpret_cast<uint4*>(dst + v1 * 16) = same ? u1 : pack8<T>(x1);
+        *reinterpret_cast<uint4*>(dst + v0 * 16) = copied ? u0 : pack8<T>(x0);
+        *reinterpret_cast<uint4*>(dst + v1 * 16) = copied ? u1 : pack8<T>(x1);
       }
-    }
-    const int hn = h + hstep;
-    if (mine && hn < heads) {
-      u0 = ld_stream16(yr + (hn * a.D + v0 * 8) * 2);
-      u1 = ld_stream16(yr + (hn * a.D + v1 * 8) * 2);
     }
   }
 }
