@@ -899,7 +899,8 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
   auto go = [&](auto t, auto d, auto nh) -> int {
     using T = decltype(t);
     constexpr int D = decltype(d)::value, NH = decltype(nh)::value;
-    constexpr int smem4 = PagedCfg<D, NH, 4>::kSmem, smem8 = PagedCfg<D, NH, 8>::kSmem;
+    constexpr int smem4 = PagedCfg<D, 4, false>::kSmem, smem8 = PagedCfg<D, 8, false>::kSmem,
+                  smem_line = PagedCfg<D, 4, true>::kSmem;
     if constexpr ((D) < 256)
       if (plan.cluster && plan.nw == 8) {
         if (!smem_configured<paged_attn_kernel<T, D, NH, 8, false>>(smem8)) return FDL_E_NODEVICE;
@@ -909,8 +910,8 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
       if (!smem_configured<paged_attn_kernel<T, D, NH, 4, false>>(smem4)) return FDL_E_NODEVICE;
       return launch_after(paged_attn_kernel<T, D, NH, 4, false>, plan.grid, 128, smem4, s, plan.cluster, a);
     }
-    if (!smem_configured<paged_attn_kernel<T, D, NH, 4, true>>(smem4)) return FDL_E_NODEVICE;
-    const int rc = launch_after(paged_attn_kernel<T, D, NH, 4, true>, plan.grid, 128, smem4, s, 1, a);
+    if (!smem_configured<paged_attn_kernel<T, D, NH, 4, true>>(smem_line)) return FDL_E_NODEVICE;
+    const int rc = launch_after(paged_attn_kernel<T, D, NH, 4, true>, plan.grid, 128, smem_line, s, 1, a);
     if (rc != FDL_OK) return rc;
     // At most one open unit a CTA.  With few units each has many pieces, and
     // fewer joining CTAs get more warps (one 65k-key sequence: 74 pieces a

@@ -71,9 +71,14 @@ constexpr int kPagedLineTile = kPagedLineWarps * kPagedWarpKeys;
 // down to a new one (p <= 256 in either 16-bit type).
 constexpr float kPagedSlack = 8.f;
 
-template <int D, int NH, int NW>
+// Stages of a warp's ring.  On the line two CTAs a SM (D = 128) with three
+// stages keep HBM busy (30.7 us for 65k keys against 31.7 us with three CTAs
+// of two stages); CTAs with a unit of their own wait on their own arithmetic,
+// and more of them with two stages win (200 rows of 1 to 1000 keys 21.8
+// against 25.1 us).
+template <int D, int NW, bool LINE>
 struct PagedCfg {
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStages = D == 128 && !LINE && NW == 4 ? 2 : 3;
   static constexpr int kStage = 2 * kPagedWarpKeys * D * 2;  // bytes of a warp's tile: K rows, V rows
   static constexpr int kSmem = NW * kStages * kStage;
 };
@@ -155,7 +160,7 @@ struct PagedPos {
 
 template <typename T, int D, int NH, int NW, bool LINE>
 __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
-  using Cfg = PagedCfg<D, NH, NW>;
+  using Cfg = PagedCfg<D, NW, LINE>;
   constexpr int kThreads = NW * 32, kTile = NW * kPagedWarpKeys;
   constexpr int kStages = Cfg::kStages, kChunks = D / 8, kRowB = D * 2, H = 8 * NH;
   constexpr int kLoads = kPagedWarpKeys * kChunks / 32;  // 16-byte pieces of K (and of V) a lane and tile
@@ -179,10 +184,12 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
     const int per = (a.B + kThreads - 1) / kThreads;
     const int b0 = threadIdx.x * per, b1 = min(a.B, b0 + per);
     long long sum = 0;
+    int one = 0;  // the length, where the thread has one sequence
     for (int b = b0; b < b1; ++b) {
       const int raw = a.lens[b];
       if (blockIdx.x == 0 && (raw < 0 || raw > a.cap)) report(FDL_DEV_LENGTH, b);
-      sum += (min(max(raw, 0), a.cap) + kTile - 1) / kTile;
+      one = min(max(raw, 0), a.cap);
+      sum += (one + kTile - 1) / kTile;
     }
     long long incl = sum;
 #pragma unroll
@@ -199,19 +206,25 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
       total += s_scan[w];
     }
     total *= a.NU;
-    // no CTA before the last busy one is without tiles, so pieces of a unit
-    // lie on consecutive CTAs
-    const long long busy = min(static_cast<long long>(gridDim.x), total);
+    // Equal pieces, the first ones a tile longer.  No CTA before the last
+    // busy one is without tiles, so pieces of a unit lie on consecutive CTAs.
     long long first = 0;
-    left = 0;
-    if (blockIdx.x < busy) {
-      first = total * blockIdx.x / busy;
-      left = static_cast<int>(total * (blockIdx.x + 1) / busy - first);
+    {
+      long long q, r;
+      if (total <= INT32_MAX) {  // 32-bit division: a tenth of the 64-bit one's instructions
+        q = static_cast<uint32_t>(total) / gridDim.x;
+        r = static_cast<uint32_t>(total) % gridDim.x;
+      } else {
+        q = total / gridDim.x;
+        r = total % gridDim.x;
+      }
+      first = q * blockIdx.x + min(static_cast<long long>(blockIdx.x), r);
+      left = static_cast<int>(q) + (blockIdx.x < r);
     }
     long long at = (incl - sum) * a.NU;
     if (left > 0 && first >= at && first < incl * a.NU) {
       for (int b = b0; b < b1; ++b) {
-        const int len = paged_len(a, b), nt = (len + kTile - 1) / kTile;
+        const int len = per == 1 ? one : paged_len(a, b), nt = (len + kTile - 1) / kTile;
         const long long mine = static_cast<long long>(nt) * a.NU;
         if (first < at + mine) {
           const int local = static_cast<int>(first - at);
