@@ -9,6 +9,8 @@ that builds it.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from pathlib import Path
 
@@ -60,6 +62,7 @@ def count_launches(n: int = 1) -> None:
 
 _abi: ctypes.CDLL | None = None
 _ops_loaded = False
+_direct = None
 
 
 def _missing(path: Path) -> ImportError:
@@ -95,7 +98,7 @@ def abi() -> ctypes.CDLL:
 
 def ensure_ops() -> None:
     """Register torch.ops.fdl.* (idempotent)."""
-    global _ops_loaded
+    global _ops_loaded, _direct
     if _ops_loaded:
         return
     abi()  # libfdl_torch.so resolves its C-ABI symbols from the loaded library
@@ -107,7 +110,21 @@ def ensure_ops() -> None:
         import torch
 
         torch.ops.load_library(str(LIB_TORCH))
+        # The same library as a Python module: its operators for plain CUDA
+        # tensors without the dispatcher (see direct()).
+        loader = importlib.machinery.ExtensionFileLoader(LIB_TORCH.stem, str(LIB_TORCH))
+        spec = importlib.util.spec_from_loader(LIB_TORCH.stem, loader)
+        _direct = importlib.util.module_from_spec(spec)
         _ops_loaded = True
+
+
+def direct():
+    """The native module whose functions take plain CUDA tensors straight into
+    the operators of torch.ops.fdl, or return NotImplemented where the call has
+    to go through the dispatcher (tensor subclasses, dispatch modes)."""
+    if _direct is None:
+        ensure_ops()
+    return _direct
 
 
 def version() -> str:

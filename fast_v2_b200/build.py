@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -72,14 +73,14 @@ def build_torch(force: bool = False, verbose: bool = False) -> Path:
     from torch.utils import cpp_extension as ce
 
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    incs = ce.include_paths(device_type="cuda")
+    incs = ce.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"]]
     libdirs = ce.library_paths(device_type="cuda")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-DTORCH_API_INCLUDE_EXTENSION_H", str(CSRC / "torch_ops.cpp"), "-o", str(LIB_TORCH) + ".tmp"]
     cmd += [f"-I{d}" for d in incs]
     cmd += [f"-L{d}" for d in libdirs]
     cmd += [f"-L{PKG}", "-lfdl_b200", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-            "-ltorch_cuda", "-lcudart"]
+            "-ltorch_cuda", "-ltorch_python", "-lcudart"]
     _run(cmd, verbose)
     os.replace(str(LIB_TORCH) + ".tmp", LIB_TORCH)
     return LIB_TORCH

@@ -24,10 +24,22 @@ import math
 from typing import Optional
 
 import torch
+from torch.compiler import is_compiling
 
 from . import _lib
 
 MAX_BATCH = 4096
+
+
+def _call(name: str, *args) -> None:
+    """An operator without a result: straight into the library for plain CUDA
+    tensors, through torch.ops.fdl otherwise and while compiling."""
+    if is_compiling():
+        getattr(torch.ops.fdl, name)(*args)
+        return
+    if getattr(_lib.direct(), name)(*args) is NotImplemented:
+        getattr(torch.ops.fdl, name)(*args)
+    _lib.count_launches(1)
 
 
 def build_slots(lens, n_new, block_table, free_pages, free_count, page_size: int, slots, positions, cu_seqlens,
@@ -45,10 +57,8 @@ def build_slots(lens, n_new, block_table, free_pages, free_count, page_size: int
     row or in ``slots``) is refused whole and reported in the device status:
     slots -1, its length unchanged.
     """
-    _lib.ensure_ops()
-    torch.ops.fdl.page_slots.default(lens, n_new, block_table, free_pages, free_count, page_size, slots, positions,
-                                     cu_seqlens, new_lens, new_count)
-    _lib.count_launches(1)
+    _call("page_slots", lens, n_new, block_table, free_pages, free_count, page_size, slots, positions, cu_seqlens,
+          new_lens, new_count)
 
 
 def release_pages(done, lens, block_table, free_pages, free_count, page_size: int) -> None:
@@ -102,10 +112,8 @@ def norm_rope_store(y, positions, inv_freq, q, k_pages, v_pages, slots, *, q_wei
     interleaved: pairs (2j, 2j + 1) instead of (j, j + rot / 2).  fp32
     arithmetic, one rounding; the angle of a far position is exact (fp64).
     """
-    _lib.ensure_ops()
-    torch.ops.fdl.norm_rope_store.default(y, positions, inv_freq, q_weight, k_weight, eps, interleaved, rope_scale, q,
-                                          k_pages, v_pages, slots)
-    _lib.count_launches(1)
+    _call("norm_rope_store", y, positions, inv_freq, q_weight, k_weight, eps, interleaved, rope_scale, q, k_pages,
+          v_pages, slots)
 
 
 def decode_attention(q, k_pages, v_pages, block_table, lens, scale: Optional[float] = None, out=None):
@@ -113,12 +121,10 @@ def decode_attention(q, k_pages, v_pages, block_table, lens, scale: Optional[flo
     D 64, 128 or 256), over the first lens[b] (int32 [B]) tokens of its pages
     [num_pages, page_size, hkv, D].  Returns [B, hq, D] (``out`` if given);
     a sequence of length 0 gives zeros.  scale: D ** -0.5 if not given."""
-    _lib.ensure_ops()
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    torch.ops.fdl.paged_decode_attn.default(q, k_pages, v_pages, block_table, lens,
-                                            q.shape[-1] ** -0.5 if scale is None else scale, out)
-    _lib.count_launches(1)
+    _call("paged_decode_attn", q, k_pages, v_pages, block_table, lens, q.shape[-1] ** -0.5 if scale is None else scale,
+          out)
     return out
 
 

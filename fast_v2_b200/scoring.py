@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.compiler import is_compiling
 
 from . import _lib
 
@@ -34,13 +35,20 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0) ->
     probability 0.  A row that is no distribution (NaN, +inf, all -inf) comes
     out as NaN with tokens -1, and is reported in the device status.
     """
-    _lib.ensure_ops()
     if logits.dim() != 2:
         raise ValueError(f"token_logprobs: logits must be [rows, vocab], got {tuple(logits.shape)}")
     if not 0 <= top <= min(MAX_TOP, logits.shape[1]):
         raise ValueError(f"token_logprobs: top={top} is outside [0, min({MAX_TOP}, vocab={logits.shape[1]})]")
-    logprob, entropy, top_logprob, top_token = torch.ops.fdl.token_logprobs.default(logits, targets, top)
-    _lib.count_launches(1)
+    # straight into the library for plain CUDA tensors, through torch.ops.fdl
+    # otherwise and while compiling
+    if is_compiling():
+        r = torch.ops.fdl.token_logprobs(logits, targets, top)
+    else:
+        r = _lib.direct().token_logprobs(logits, targets, top)
+        if r is NotImplemented:
+            r = torch.ops.fdl.token_logprobs(logits, targets, top)
+        _lib.count_launches(1)
+    logprob, entropy, top_logprob, top_token = r
     if not top:
         top_logprob = top_token = None
     return TokenScores(logprob, entropy, top_logprob, top_token)

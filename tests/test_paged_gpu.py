@@ -535,3 +535,68 @@ def test_a_serving_run(dt, graph):
     assert int(cache.free_count[0]) == 40 - held
     pages = [p for row in cache.block_table.tolist() for p in row if p >= 0]
     assert len(pages) == held and sorted(pages + cache.free_pages[: 40 - held].tolist()) == list(range(40))
+
+
+# ------------------------------------------------------------------ ways to call
+class _Sub(torch.Tensor):
+    """A subclass without behaviour of its own: calls go through torch.ops."""
+
+
+def test_direct_and_dispatched_calls_agree():
+    a = _attn_case(1, [300, 20, 500], 28, 4, 128, 16, BF)
+    want = paged.decode_attention(*a)
+    out = torch.empty_like(want)
+    assert _lib.direct().paged_decode_attn(*a, 128 ** -0.5, out) is None  # plain tensors need no dispatcher
+    assert torch.equal(out, want)
+    assert _lib.direct().paged_decode_attn(a[0].as_subclass(_Sub), *a[1:], 128 ** -0.5, out) is NotImplemented
+    out.zero_()
+    torch.ops.fdl.paged_decode_attn(*a, 128 ** -0.5, out)
+    assert torch.equal(out, want)
+    out.zero_()
+    paged.decode_attention(a[0].as_subclass(_Sub), *a[1:], out=out)
+    assert torch.equal(out, want)
+    x = torch.randn(9, 1000, device=DEV)
+    t = torch.arange(9, device=DEV)
+    r = scoring.token_logprobs(x, t, 3)
+    for other in (torch.ops.fdl.token_logprobs(x, t, 3), scoring.token_logprobs(x.as_subclass(_Sub), t, 3)):
+        for u, v in zip(r, other):
+            assert torch.equal(u, torch.Tensor(v) if isinstance(v, _Sub) else v)
+    assert all(not u.requires_grad for u in r)
+
+
+def test_compiled_calls():
+    a = _attn_case(1, [300, 20, 500], 28, 4, 128, 16, BF)
+    x = torch.randn(9, 1000, device=DEV)
+    t = torch.arange(9, device=DEV)
+
+    def f(a, x, t):
+        o = paged.decode_attention(*a)
+        r = scoring.token_logprobs(x * 2, t, 3)
+        return o + 1, r.logprob, r.top_token
+
+    want = f(a, x, t)
+    got = torch.compile(f, fullgraph=True, backend="aot_eager")(a, x, t)
+    for u, v in zip(want, got):
+        assert torch.equal(u, v)
+
+
+def test_calls_from_threads():
+    import threading
+
+    a = _attn_case(1, [300, 20, 500], 28, 4, 128, 16, BF)
+    want = paged.decode_attention(*a)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not torch.equal(paged.decode_attention(*a), want):
+                    bad.append(1)
+
+    ts = [threading.Thread(target=work) for _ in range(4)]
+    for th in ts:
+        th.start()
+    for th in ts:
+        th.join()
+    assert not bad
