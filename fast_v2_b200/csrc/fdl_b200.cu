@@ -776,7 +776,7 @@ int fdl_page_slots(const int32_t* lens, const int32_t* n_new, int batch, int32_t
                    int64_t* positions, int64_t n_rows, int32_t* cu, int32_t* new_lens, int32_t* new_count,
                    fdl_stream_t stream) {
   if (batch < 1 || batch > kSlotsMaxBatch || max_pages < 0 || n_free < 0 || page_size < 1 || n_rows < 0 ||
-      n_rows > INT32_MAX || table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+      n_rows > INT32_MAX || table_sb < max_pages || (static_cast<int64_t>(max_pages) + 1) * page_size > INT32_MAX)
     return FDL_E_SHAPE;
   if (!lens || !n_new || !count || !cu || !new_lens || !new_count || (max_pages > 0 && !table) ||
       (n_free > 0 && !free_pages) || (n_rows > 0 && (!slots || !positions)))
@@ -793,7 +793,7 @@ int fdl_page_slots(const int32_t* lens, const int32_t* n_new, int batch, int32_t
 int fdl_page_release(const uint8_t* done, int32_t* lens, int batch, int32_t* table, int64_t table_sb, int max_pages,
                      int32_t* free_pages, int n_free, int32_t* count, int page_size, fdl_stream_t stream) {
   if (batch < 1 || batch > kSlotsMaxBatch || max_pages < 0 || n_free < 0 || page_size < 1 || table_sb < max_pages ||
-      static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+      (static_cast<int64_t>(max_pages) + 1) * page_size > INT32_MAX)
     return FDL_E_SHAPE;
   if (!done || !lens || !count || (max_pages > 0 && !table) || (n_free > 0 && !free_pages)) return FDL_E_NULL;
   PageReleaseArgs a{done, lens, table, table_sb, free_pages, count, batch, max_pages, n_free, {}};
@@ -816,6 +816,8 @@ int fdl_norm_rope_store(const void* y, int64_t y_rs, const int64_t* pos, const f
   if (width > (1 << 24) || (rows > 1 && y_rs < width)) return FDL_E_SHAPE;
   if (rows == 0) return FDL_OK;
   if (!y || !pos || (n_freq > 0 && !inv_freq) || !q || !k_pages || !v_pages || !slots) return FDL_E_NULL;
+  if (k_pages == v_pages || (hkv > 1 && kv_sh == 0) || (page_size > 1 && kv_ss == 0) || (num_pages > 1 && kv_sp == 0))
+    return FDL_E_SHAPE;  // two rows would share memory
   for (const void* p : {y, static_cast<const void*>(q), static_cast<const void*>(k_pages),
                         static_cast<const void*>(v_pages), q_weight, k_weight})
     if (!aligned16(p)) return FDL_E_ALIGN;
@@ -871,7 +873,7 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
                    fdl_stream_t stream) {
   if (dtype != FDL_BF16 && dtype != FDL_F16) return FDL_E_DTYPE;
   if (batch < 0 || batch > 65535 || hq < 1 || hq > 4096 || hkv < 1 || hq % hkv || num_pages < 0 || page_size < 1 ||
-      max_pages < 0 || table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX - 1024)
+      max_pages < 0 || (num_pages == 0 && max_pages > 0) || table_sb < max_pages || static_cast<int64_t>(max_pages) * page_size > INT32_MAX - 1024)
     return FDL_E_SHAPE;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FDL_E_UNSUPPORTED;
   if (batch == 0) return FDL_OK;
@@ -940,7 +942,7 @@ int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int voc
                        float* logprob, float* entropy, int top, float* top_logprob, int64_t* top_token,
                        fdl_stream_t stream) {
   if (dtype != FDL_BF16 && dtype != FDL_F16 && dtype != FDL_F32) return FDL_E_DTYPE;
-  if (rows < 0 || vocab < 1 || row_stride < vocab || top < 0 || top > kTokMaxTop || top > vocab) return FDL_E_SHAPE;
+  if (rows < 0 || vocab < 1 || row_stride < 0 || top < 0 || top > kTokMaxTop || top > vocab) return FDL_E_SHAPE;
   if (rows == 0) return FDL_OK;
   if (!logits || !targets || !logprob || !entropy || (top > 0 && (!top_logprob || !top_token))) return FDL_E_NULL;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == FDL_F32 ? 4 : 2)) return FDL_E_ALIGN;

@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
   const bool whole = a.page.d % kPagedWarpKeys == 0;  // the 16 keys lie in one page
   const int64_t lane_src = static_cast<int64_t>(lane / kChunks) * a.ss + (lane % kChunks) * 16;
   const int64_t step_src = a.ss * kRows;
-  const int64_t v_minus_k = a.v - a.k;
+  const int64_t v_minus_k = reinterpret_cast<int64_t>(a.v) - reinterpret_cast<int64_t>(a.k);
   // Row r holds its 16-byte piece ch at ch ^ (r & 7): eight rows of one piece
   // lie in different banks.  Offsets of this lane, by what they depend on.
   uint32_t to_off[8 / kRows], k_off[4], v_off[4];

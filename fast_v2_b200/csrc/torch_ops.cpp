@@ -755,8 +755,9 @@ void paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.stride(2) == 1,
               "fdl.paged_decode_attn: q must be a CUDA [B, hq, D] tensor, contiguous in D");
   TORCH_CHECK(out.is_cuda() && out.device() == q.device() && out.dtype() == q.dtype() && out.sizes() == q.sizes() &&
-                  out.stride(2) == 1,
-              "fdl.paged_decode_attn: out must match q, contiguous in D");
+                  out.stride(2) == 1 && (out.size(0) <= 1 || out.stride(0) != 0) &&
+                  (out.size(1) <= 1 || out.stride(1) != 0),
+              "fdl.paged_decode_attn: out must match q, contiguous in D and with memory of its own for each row");
   check_pages(k_pages, v_pages, q, "paged_decode_attn");
   const int64_t B = q.size(0), hq = q.size(1), D = q.size(2), hkv = k_pages.size(2), page = k_pages.size(1);
   TORCH_CHECK(k_pages.size(3) == D && hkv >= 1 && hq % hkv == 0, "fdl.paged_decode_attn: q ", q.sizes(),

@@ -39,7 +39,6 @@ def _call(name: str, *args) -> None:
         return
     if getattr(_lib.direct(), name)(*args) is NotImplemented:
         getattr(torch.ops.fdl, name)(*args)
-    _lib.count_launches(1)
 
 
 def build_slots(lens, n_new, block_table, free_pages, free_count, page_size: int, slots, positions, cu_seqlens,
@@ -65,8 +64,7 @@ def release_pages(done, lens, block_table, free_pages, free_count, page_size: in
     """Return the pages of the sequences with ``done[b]`` (bool [B]) to the
     pool; their table entries become -1 and their lengths 0."""
     _lib.ensure_ops()
-    torch.ops.fdl.page_release.default(done, lens, block_table, free_pages, free_count, page_size)
-    _lib.count_launches(1)
+    torch.ops.fdl.page_release(done, lens, block_table, free_pages, free_count, page_size)
 
 
 def rope_frequencies(rot_dim: int, base: float = 1e6, *, factor: float = 1.0, original_len: Optional[int] = None,
@@ -111,6 +109,7 @@ def norm_rope_store(y, positions, inv_freq, q, k_pages, v_pages, slots, *, q_wei
 
     interleaved: pairs (2j, 2j + 1) instead of (j, j + rot / 2).  fp32
     arithmetic, one rounding; the angle of a far position is exact (fp64).
+    q may not share memory with y, nor two rows a slot.
     """
     _call("norm_rope_store", y, positions, inv_freq, q_weight, k_weight, eps, interleaved, rope_scale, q, k_pages,
           v_pages, slots)

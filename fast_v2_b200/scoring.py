@@ -29,7 +29,8 @@ class TokenScores(NamedTuple):
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0) -> TokenScores:
     """Log probability of ``targets`` (int64, one per row; below 0: no target,
     scored 0), entropy and the ``top`` <= 32 best tokens of ``logits``
-    [rows, vocab] (bf16, fp16 or fp32; rows may be strided).
+    [rows, vocab] (bf16, fp16 or fp32; rows may be strided, or one row
+    expanded to score several targets).
 
     Equal logits rank by index, lower first.  -inf logits are tokens of
     probability 0.  A row that is no distribution (NaN, +inf, all -inf) comes
@@ -47,7 +48,6 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0) ->
         r = _lib.direct().token_logprobs(logits, targets, top)
         if r is NotImplemented:
             r = torch.ops.fdl.token_logprobs(logits, targets, top)
-        _lib.count_launches(1)
     logprob, entropy, top_logprob, top_token = r
     if not top:
         top_logprob = top_token = None

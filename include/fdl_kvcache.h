@@ -460,7 +460,8 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
  * pages or rows that run out) is refused whole: slots -1, length unchanged, no
  * page taken, FDL_DEV_LENGTH (info = b); sequences behind it that need pages
  * are refused with it when the pool is what ran out.  Rows behind the last
- * token get slot -1 and position 0.  batch <= 4096.
+ * token get slot -1 and position 0.  batch <= 4096, (max_pages + 1) *
+ * page_size < 2^31.
  *
  * fdl_page_release: for every b with done[b] (bytes, 0 or 1) the pages of the
  * sequence go back onto the stack, its table entries become -1, its length 0.
@@ -477,14 +478,14 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
  * [rows]; -1 stores nothing, any other slot outside the pool stores nothing
  * and is reported).  Two rows may not name one slot.  All arithmetic is fp32
  * (the angle fp64), rounded once.  bf16 or f16; D % 16 == 0, D <= 256, n_freq
- * % 8 == 0, 2 * n_freq <= D.  Unlike fdl_rope_qkv_kv, which repeats the
- * reference's bf16 roundings.
+ * % 8 == 0, 2 * n_freq <= D.  q must not overlap y, k_pages not v_pages.
+ * Unlike fdl_rope_qkv_kv, which repeats the reference's bf16 roundings.
  *
  * fdl_paged_attn: attention of one query token per sequence,
  *   out[b, h] = softmax_j(scale * q[b, h] . K[b, j, h / (hq / hkv)]) V[b, j, ..]
  * over keys j < lens[b] (clamped to the table's width, FDL_DEV_LENGTH).  q and
- * out [B, hq, D] with strides; bf16 or f16, D 64, 128 or 256.  A sequence
- * without keys gives zeros.  A page outside [0, num_pages) hides its keys and
+ * out [B, hq, D] with strides; bf16 or f16, D 64, 128 or 256, hq <= 4096, any
+ * hq / hkv.  A sequence without keys gives zeros.  A page outside [0, num_pages) hides its keys and
  * is reported.  Softmax in fp32.  workspace: at least
  * fdl_paged_attn_workspace_bytes() bytes, 16-byte aligned, not shared with a
  * call that may run at the same time; its contents need not be kept.
@@ -523,7 +524,7 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh,
 
 /* ------------------------------------------------------------------------
  * Scores of given tokens over the vocabulary: for every row of logits [rows,
- * vocab] (bf16, f16 or f32, row stride in elements, any alignment),
+ * vocab] (bf16, f16 or f32, row stride in elements, 0 allowed, any alignment),
  *   lse = ln sum_v exp(l_v),  logprob[r] = l_target - lse,
  *   entropy[r] = -sum_v p_v ln p_v,  p_v = exp(l_v - lse),
  *   top_token[r, :top], top_logprob[r, :top] = the top tokens of largest

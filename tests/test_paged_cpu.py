@@ -39,7 +39,8 @@ SLOTS_T = [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, i64, vp, vp, vp,
 @pytest.mark.parametrize("change,rc", [
     (dict(batch=0), SHAPE), (dict(batch=4097), SHAPE), (dict(page=0), SHAPE), (dict(max_pages=-1), SHAPE),
     (dict(table_sb=3), SHAPE), (dict(n_free=-1), SHAPE), (dict(n_rows=-1), SHAPE), (dict(n_rows=1 << 31), SHAPE),
-    (dict(max_pages=1 << 20, table_sb=1 << 20, page=1 << 12), SHAPE), (dict(lens=None), NULL),
+    (dict(max_pages=1 << 20, table_sb=1 << 20, page=1 << 12), SHAPE),
+    (dict(max_pages=1, table_sb=1, page=1 << 30), SHAPE), (dict(lens=None), NULL),
     (dict(n_new=None), NULL), (dict(table=None), NULL), (dict(free_pages=None), NULL), (dict(count=None), NULL),
     (dict(slots=None), NULL), (dict(positions=None), NULL), (dict(cu=None), NULL), (dict(new_lens=None), NULL),
     (dict(new_count=None), NULL)])
@@ -54,13 +55,13 @@ RELEASE_T = [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp]
 
 @pytest.mark.parametrize("change,rc", [
     (dict(batch=0), SHAPE), (dict(batch=4097), SHAPE), (dict(page=0), SHAPE), (dict(table_sb=3), SHAPE),
-    (dict(done=None), NULL), (dict(lens=None), NULL), (dict(table=None), NULL), (dict(free_pages=None), NULL),
+    (dict(max_pages=1, table_sb=1, page=1 << 30), SHAPE), (dict(done=None), NULL), (dict(lens=None), NULL), (dict(table=None), NULL), (dict(free_pages=None), NULL),
     (dict(count=None), NULL)])
 def test_page_release_refusals(change, rc):
     assert _call("fdl_page_release", RELEASE_T, RELEASE, change) == rc
 
 
-ROPE = dict(y=P, y_rs=1536, pos=P, inv_freq=P, n_freq=64, qw=P, kw=P, eps=1e-6, inter=0, scale=1.0, q=P, k=P, v=P,
+ROPE = dict(y=P, y_rs=1536, pos=P, inv_freq=P, n_freq=64, qw=P, kw=P, eps=1e-6, inter=0, scale=1.0, q=P, k=P, v=2 * P,
             sp=4096, ss=256, sh=128, num_pages=8, page=16, slots=P, rows=4, hq=8, hkv=2, dim=128, dtype=BF16,
             stream=None)
 ROPE_T = [vp, i64, vp, vp, i32, vp, vp, f32, i32, f32, vp, vp, vp, i64, i64, i64, i32, i32, vp, i64, i32, i32, i32,
@@ -73,7 +74,8 @@ ROPE_T = [vp, i64, vp, vp, i32, vp, vp, f32, i32, f32, vp, vp, vp, i64, i64, i64
     (dict(dim=120), SHAPE), (dict(dim=8), SHAPE), (dict(dim=272), SHAPE), (dict(n_freq=65), SHAPE),
     (dict(n_freq=12), SHAPE), (dict(n_freq=72), SHAPE), (dict(n_freq=-8), SHAPE), (dict(num_pages=0), SHAPE),
     (dict(page=0), SHAPE), (dict(num_pages=1 << 20, page=1 << 12), SHAPE), (dict(y_rs=1528), SHAPE),
-    (dict(hq=1 << 30, hkv=1 << 29, y_rs=1 << 60), SHAPE), (dict(y=None), NULL), (dict(pos=None), NULL),
+    (dict(hq=1 << 30, hkv=1 << 29, y_rs=1 << 60), SHAPE), (dict(v=P), SHAPE), (dict(sh=0), SHAPE), (dict(ss=0), SHAPE),
+    (dict(sp=0), SHAPE), (dict(y=None), NULL), (dict(pos=None), NULL),
     (dict(inv_freq=None), NULL), (dict(q=None), NULL), (dict(k=None), NULL), (dict(v=None), NULL),
     (dict(slots=None), NULL), (dict(y=P + 2), ALIGN), (dict(q=P + 8), ALIGN), (dict(k=P + 2), ALIGN),
     (dict(v=P + 4), ALIGN), (dict(qw=P + 2), ALIGN), (dict(kw=P + 2), ALIGN), (dict(y_rs=1540), ALIGN),
@@ -92,7 +94,7 @@ ATTN_T = [vp, i64, i64, vp, vp, i64, i64, i64, i32, i32, vp, i64, i32, vp, i32, 
 @pytest.mark.parametrize("change,rc", [
     (dict(batch=0), OK), (dict(dtype=F32), DTYPE), (dict(batch=-1), SHAPE), (dict(batch=65536), SHAPE),
     (dict(hq=0), SHAPE), (dict(hkv=0), SHAPE), (dict(hq=9), SHAPE), (dict(page=0), SHAPE), (dict(num_pages=-1), SHAPE),
-    (dict(max_pages=-1), SHAPE), (dict(table_sb=3), SHAPE),
+    (dict(max_pages=-1), SHAPE), (dict(table_sb=3), SHAPE), (dict(num_pages=0), SHAPE), (dict(hq=8192), SHAPE),
     (dict(max_pages=1 << 20, table_sb=1 << 20, page=1 << 12), SHAPE), (dict(dim=96), UNSUPPORTED),
     (dict(dim=512), UNSUPPORTED), (dict(q=None), NULL), (dict(k=None), NULL), (dict(v=None), NULL),
     (dict(table=None), NULL), (dict(lens=None), NULL), (dict(out=None), NULL), (dict(q=P + 2), ALIGN),
@@ -110,7 +112,7 @@ SCORE_T = [vp, i64, i32, i32, i32, vp, vp, vp, i32, vp, vp, vp]
 
 @pytest.mark.parametrize("change,rc", [
     (dict(rows=0), OK), (dict(rows=0, x=None), OK), (dict(dtype=3), DTYPE), (dict(rows=-1), SHAPE),
-    (dict(vocab=0, rs=0), SHAPE), (dict(rs=999), SHAPE), (dict(top=-1), SHAPE), (dict(top=33), SHAPE),
+    (dict(vocab=0, rs=0), SHAPE), (dict(rs=-1), SHAPE), (dict(top=-1), SHAPE), (dict(top=33), SHAPE),
     (dict(vocab=4, top=5), SHAPE), (dict(x=None), NULL), (dict(targets=None), NULL), (dict(lp=None), NULL),
     (dict(ent=None), NULL), (dict(top_lp=None), NULL), (dict(top_tok=None), NULL), (dict(x=P + 1), ALIGN),
     (dict(dtype=F32, x=P + 2), ALIGN)])

@@ -177,3 +177,49 @@ def test_refusals_and_empty_rows():
             scoring.token_logprobs(*args)
     r = scoring.token_logprobs(x[:0], t[:0], 3)
     assert r.logprob.shape == (0,) and r.top_token.shape == (0, 3)
+
+
+def test_one_row_expanded_for_several_targets():
+    x, _ = _logits(9, 1, 3001, BF)
+    t = torch.arange(0, 3001, 300, device=DEV)
+    got = _check(x.expand(t.numel(), 3001), t, 2)
+    # one row at one address: the same sums for every target
+    assert bool((got.entropy == got.entropy[0]).all()) and bool((got.top_token == got.top_token[0]).all())
+
+
+@pytest.mark.parametrize("dt,V,top", [(BF, 1000, 20), (HF, 3500, 32), (F, 5119, 5), (BF, 250, 8), (BF, 48001, 20),
+                                      (F, 20001, 32)])
+def test_scores_of_many_rows(dt, V, top):
+    """The forms for many rows: a warp a row, half a CTA a row."""
+    x, t = _logits(V, 1300, V, dt)
+    t[::7] = -1
+    x[3] = -math.inf
+    x[3, V // 2] = 1.0
+    t[3] = V // 2
+    x[4] = 0.25                          # all equal
+    x[5, : V // 2] = torch.finfo(dt).min  # a mask of the lowest value
+    x[6] = torch.finfo(dt).min
+    t[5] = V - 1
+    _check(x, t, top)
+    x[7, V - 1] = float("nan")
+    got = scoring.token_logprobs(x, t, top)
+    assert _lib.last_device_error() == (1, 7)
+    assert bool(got.logprob[7].isnan()) and got.top_token[7].tolist() == [-1] * top
+
+
+@pytest.mark.parametrize("rows", [2, 700])
+@pytest.mark.parametrize("dt", [BF, HF, F])
+def test_scores_under_masks_of_the_lowest_value(rows, dt):
+    V = 9000
+    x, t = _logits(rows, rows, V, dt)
+    low = torch.finfo(dt).min
+    x[:, 100:8900] = low
+    t.fill_(8950)
+    _check(x, t, 32)
+    x[0] = low                            # nothing but the mask: every token alike
+    t[0] = 5
+    _check(x, t, 7)
+    x[1, :] = -math.inf
+    x[1, 17] = low
+    t[1] = 17
+    _check(x, t, 3)
