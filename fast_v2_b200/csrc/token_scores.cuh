@@ -434,9 +434,16 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
       if (in && !more)
         for (int i = pass.at; i <= pass.last(); i += NT) offer_vector(i);
       if (single >= 0) offer(lone, single);
-      // the warp reads all vectors of such a thread
-      for (unsigned who = __ballot_sync(0xffffffffu, more); who; who &= who - 1)
-        for (int i = warp * 32 + __ffs(who) - 1 + lane * NT; i < nv; i += 32 * NT) offer_vector(i);
+      // the warp reads all vectors of such threads, all lanes at work
+      const unsigned who = __ballot_sync(0xffffffffu, more);
+      const int each = (nv + NT - 1) / NT;
+      for (int p = lane; p < __popc(who) * each; p += 32) {
+        unsigned w = who;
+        int i = p;
+        for (; i >= each; i -= each) w &= w - 1;
+        i = warp * 32 + __ffs(w) - 1 + i * NT;
+        if (i < nv) offer_vector(i);
+      }
       __syncthreads();
       const int n = sh_n;
       block_rank<NT>(sh_cand, min(n, kTokList), sh_top);
@@ -478,20 +485,31 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
       }
       row_s = TokSums{to, __shfl_sync(0xffffffffu, o.z, 0), __shfl_sync(0xffffffffu, o.t, 0)};
       if (a.top > 0) {
+        // The largest of the CTAs' k-th best is a tau for the row; what is
+        // below it need not be ranked.
         const int n = static_cast<int>(ranks) * a.top;
-        for (int i = threadIdx.x; i < n; i += NT) {
-          const float2 k2 = ld_cluster2(smem_addr(&sh_top[i % a.top]), i / a.top);
-          // empty entries (a CTA with fewer than k entries) stay distinct
-          const uint64_t k = static_cast<uint64_t>(__float_as_uint(k2.y)) << 32 | __float_as_uint(k2.x);
-          sh_cand[i] = k ? k : i + 1;
+        uint64_t k = 0;
+        if (threadIdx.x < n) {  // n <= 8 * 32 = NT
+          const float2 k2 = ld_cluster2(smem_addr(&sh_top[threadIdx.x % a.top]), threadIdx.x / a.top);
+          k = static_cast<uint64_t>(__float_as_uint(k2.y)) << 32 | __float_as_uint(k2.x);
+          if (k == 0) k = threadIdx.x + 1;  // empty entries (a CTA with fewer than k entries) stay distinct
         }
+        if (threadIdx.x == 0) {
+          sh_tau = 0;
+          sh_n = 0;
+        }
+        __syncthreads();
+        if (threadIdx.x < n && threadIdx.x % a.top == a.top - 1)
+          atomicMax(reinterpret_cast<unsigned long long*>(&sh_tau), static_cast<unsigned long long>(k));
+        __syncthreads();
+        if (threadIdx.x < n && k >= sh_tau) sh_cand[atomicAdd(&sh_n, 1)] = k;
         __syncthreads();
       }
     }
     cluster_sync();  // no CTA leaves (or ranks into sh_top) while its shared memory is read
     if (rank != 0) return;
     if (a.top > 0) {
-      block_rank<NT>(sh_cand, static_cast<int>(ranks) * a.top, sh_top);
+      block_rank<NT>(sh_cand, sh_n, sh_top);
       __syncthreads();
     }
   }
