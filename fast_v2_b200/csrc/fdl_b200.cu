@@ -957,17 +957,19 @@ int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int voc
   // time is one row's: 100 of 625 vectors 8.8 (warp) against 8.0 us (cluster);
   // a cluster of 8 pays for itself below two CTAs a SM (64 rows of 19008: 14.0
   // us with 4, 18.6 with 8).
-  auto go = [&](auto t) {
+  auto go = [&](auto t) -> int {
     using T = decltype(t);
+    constexpr int kRing = kTokStages * kTokUnroll * kTokCta * 16;
+    if (!smem_configured<token_scores_kernel<T, kTokCta>>(kRing)) return FDL_E_NODEVICE;
     if (vectors <= 1280 && rows >= 4 * num_sms())
       return launch_after(token_scores_warp_kernel<T>, (rows + kTokRowWarps - 1) / kTokRowWarps, kTokRowWarps * 32, 0, s,
                           1, a);
     if (vectors <= 6144 && rows >= 8 * num_sms())
-      return launch_after(token_scores_kernel<T, kTokCta / 2>, rows, kTokCta / 2, 0, s, 1, a);
+      return launch_after(token_scores_kernel<T, kTokCta / 2>, rows, kTokCta / 2, kRing / 2, s, 1, a);
     int cluster = 1;
     while (cluster < 8 && static_cast<int64_t>(rows) * cluster < 2ll * num_sms() && vectors >= 2ll * cluster * kTokCta)
       cluster *= 2;
-    return launch_after(token_scores_kernel<T, kTokCta>, rows * cluster, kTokCta, 0, s, cluster, a);
+    return launch_after(token_scores_kernel<T, kTokCta>, rows * cluster, kTokCta, kRing, s, cluster, a);
   };
   return dtype == FDL_BF16 ? go(__nv_bfloat16{}) : dtype == FDL_F16 ? go(__half{}) : go(float{});
 }

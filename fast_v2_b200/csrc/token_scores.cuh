@@ -45,7 +45,8 @@ constexpr int kTokCta = 256;      // threads a row, or half of them
 constexpr int kTokRowWarps = 8;   // rows a CTA of the warp form
 constexpr int kTokRowList = 320;  // its lists (31 vectors of 8 entries and 14 more fit)
 constexpr int kTokList = 512;  // entries above tau that are caught (a cluster of 8 brings 8 * 32)
-constexpr int kTokUnroll = 3;  // vectors in flight a thread
+constexpr int kTokUnroll = 3;  // vectors a batch
+constexpr int kTokStages = 4;  // batches of a thread's ring
 constexpr float kTokSlack = 10.f;
 constexpr float kTokLog2e = 1.4426950408889634f;
 constexpr float kTokBig = 1048576.f;  // 2^20: its product with log2 e rounds by 2^-4 at most
@@ -236,17 +237,71 @@ struct TokPass {
 #pragma unroll
     for (int e = 0; e < kN; e += 2) sums.add(q.f[e], q.f[e + 1]);
   }
-  // The warp form reads many vectors of its short row again, so it lets them
-  // stay in L1.
-  __device__ __forceinline__ static uint4 load(const char* p) {
-    if constexpr (NT == 32) return __ldg(reinterpret_cast<const uint4*>(p));
-    return ld_stream16(p);
-  }
-  __device__ __forceinline__ void run(const char* vec, int nv, int tid) {
+  __device__ __forceinline__ void start(int nv, int tid) {
     sums.start();
     best = second = -INFINITY;
     at = tid;
     whole = nv / kBatch * kBatch;
+  }
+  __device__ __forceinline__ void batch(const uint4 (&u)[kTokUnroll], int v) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kTokUnroll; ++i) m = fmaxf(m, TokVec<T>::finite(u[i]).max());
+    note(m, v);
+#pragma unroll
+    for (int i = 0; i < kTokUnroll; ++i) add(TokVec<T>::finite(u[i]));
+  }
+  __device__ __forceinline__ void one(uint4 u, int v) {
+    const TokVec<T> q = TokVec<T>::finite(u);
+    note(q.max(), v);
+    add(q);
+  }
+  // A CTA's threads: each has a ring of kTokStages batches in shared memory,
+  // filled by its own asynchronous copies (nothing is shared, so nothing waits
+  // for another thread).  ring: kTokStages * kBatch * 16 bytes of the CTA.
+  __device__ __forceinline__ void run_ring(const char* vec, int nv, int tid, char* ring) {
+    start(nv, tid);
+    const char* src = vec + tid * 16;
+    const uint32_t dst = smem_addr(ring) + tid * 16;
+    int next = 0, fill = 0;  // first vector and slot of the next batch to load
+    auto issue = [&]() {
+      if (next < nv) {
+#pragma unroll
+        for (int i = 0; i < kTokUnroll; ++i)
+          if (next < whole || next + tid + i * NT < nv)
+            cp_async16(dst + (fill * kTokUnroll + i) * NT * 16, src + i * NT * 16);
+        src += kBatch * 16;
+        next += kBatch;
+        fill = fill + 1 == kTokStages ? 0 : fill + 1;
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kTokStages - 1; ++i) issue();
+    const uint4* mine = reinterpret_cast<const uint4*>(ring) + tid;
+    int use = 0;
+    for (int v = 0; v < nv; v += kBatch) {
+      issue();
+      cp_wait<kTokStages - 1>();
+      const uint4* slot = mine + use * kTokUnroll * NT;
+      use = use + 1 == kTokStages ? 0 : use + 1;
+      if (v < whole) {
+        uint4 u[kTokUnroll];
+#pragma unroll
+        for (int i = 0; i < kTokUnroll; ++i) u[i] = slot[i * NT];
+        batch(u, v + tid);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTokUnroll; ++i)
+          if (v + tid + i * NT < nv) one(slot[i * NT], v + tid + i * NT);
+      }
+    }
+  }
+  // The warp form reads many vectors of its short row again, so it lets them
+  // stay in L1.
+  __device__ __forceinline__ static uint4 load(const char* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void run(const char* vec, int nv, int tid) {
+    start(nv, tid);
     const char* p = vec + tid * 16;
     uint4 next[kTokUnroll];  // the next batch is on its way while one is summed
     auto fetch = [&](int v) {
@@ -266,21 +321,12 @@ struct TokPass {
 #pragma unroll
       for (int i = 0; i < kTokUnroll; ++i) u[i] = next[i];
       fetch(v + kBatch);
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kTokUnroll; ++i) m = fmaxf(m, TokVec<T>::finite(u[i]).max());
-      note(m, v + tid);
-#pragma unroll
-      for (int i = 0; i < kTokUnroll; ++i) add(TokVec<T>::finite(u[i]));
+      batch(u, v + tid);
     }
 #pragma unroll
     for (int i = 0; i < kTokUnroll; ++i) {
       const int v = whole + tid + i * NT;
-      if (v < nv) {
-        const TokVec<T> q = TokVec<T>::finite(next[i]);
-        note(q.max(), v);
-        add(q);
-      }
+      if (v < nv) one(next[i], v);
     }
   }
   // The largest entry lies between (least_order(), least_index(first)) -- the
@@ -298,6 +344,7 @@ struct TokPass {
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __grid_constant__ TokScoreArgs a) {
   constexpr int kN = TokVec<T>::kN, kWarps = NT / 32;
+  extern __shared__ __align__(16) char ring[];
   __shared__ float sh_m[kWarps], sh_z[kWarps], sh_t[kWarps];
   __shared__ uint64_t sh_max[kWarps + kTokMaxTop];  // the largest thread maxima of each warp
   __shared__ uint64_t sh_tau;
@@ -334,7 +381,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
 
   // ---- the one pass
   TokPass<T, NT> pass;
-  pass.run(vec, nv, threadIdx.x);
+  pass.run_ring(vec, nv, threadIdx.x, ring);
   TokSums s = pass.sums.natural();
   float lone = -INFINITY;
   if (single >= 0) {
