@@ -781,8 +781,11 @@ void paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
 }
 
 // Returns (logprob [rows], entropy [rows], top_logprob [rows, top], top_token
-// [rows, top]); the outputs come from torch's caching allocator.
-std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& targets, int64_t top) {
+// [rows, top]) from torch's caching allocator: a tensor each, or (`one`) four
+// parts of one allocation, which the outputs of a dispatched operator may not
+// be.
+using Scores = std::tuple<Tensor, Tensor, Tensor, Tensor>;
+Scores token_logprobs_in(const Tensor& logits, const Tensor& targets, int64_t top, bool one) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
               "fdl.token_logprobs: logits must be a CUDA [rows, vocab] tensor with unit inner stride");
   const int64_t rows = logits.size(0), V = logits.size(1);
@@ -790,11 +793,24 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
   const int code = dtype_code(logits);
   TORCH_CHECK(top >= 0 && top <= V, "fdl.token_logprobs: top is ", top, " of ", V, " tokens");
   c10::cuda::CUDAGuard guard(logits.device());
-  auto make = [&](at::IntArrayRef size, at::ScalarType type) {
+  auto empty = [&](at::IntArrayRef size, at::ScalarType type) -> Tensor {
     return at::detail::empty_cuda(size, type, logits.device(), std::nullopt);
   };
+  Tensor all;
+  int64_t used = 0;  // bytes; the 8-byte tokens come first
+  if (one) all = empty({12 * rows * top + 8 * rows}, at::kByte);
+  auto make = [&](at::IntArrayRef size, at::ScalarType type) -> Tensor {
+    if (!one) return empty(size, type);
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()),
+                                                        c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(used / static_cast<int64_t>(c10::elementSize(type)));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    used += t.numel() * static_cast<int64_t>(c10::elementSize(type));
+    return t;
+  };
+  Tensor top_tok = make({rows, top}, at::kLong), top_lp = make({rows, top}, at::kFloat);
   Tensor logprob = make({rows}, at::kFloat), entropy = make({rows}, at::kFloat);
-  Tensor top_lp = make({rows, top}, at::kFloat), top_tok = make({rows, top}, at::kLong);
   check_rc(fdl_token_logprobs(logits.data_ptr(), rows > 1 ? logits.stride(0) : V, as_int(rows, "rows"),
                               as_int(V, "the vocabulary"), code, targets.data_ptr<int64_t>(),
                               logprob.data_ptr<float>(), entropy.data_ptr<float>(), as_int(top, "top"),
@@ -803,8 +819,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
            "token_logprobs");
   return {logprob, entropy, top_lp, top_tok};
 }
+Scores token_logprobs(const Tensor& logits, const Tensor& targets, int64_t top) {
+  return token_logprobs_in(logits, targets, top, false);
+}
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs_meta(const Tensor& logits, const Tensor&, int64_t top) {
+Scores token_logprobs_meta(const Tensor& logits, const Tensor&, int64_t top) {
   const int64_t rows = logits.size(0);
   auto f = logits.options().dtype(at::kFloat);
   return {at::empty({rows}, f), at::empty({rows}, f), at::empty({rows, top}, f),
@@ -932,10 +951,10 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!direct(a, n, 3, {0, 1})) Py_RETURN_NOTIMPLEMENTED;
   const Tensor logits = tensor(a[0]), targets = tensor(a[1]);
   const int64_t top = integer(a[2]);
-  std::tuple<Tensor, Tensor, Tensor, Tensor> r;
+  Scores r;
   {
     NoGil g;
-    r = token_logprobs(logits, targets, top);
+    r = token_logprobs_in(logits, targets, top, true);
   }
   return Py_BuildValue("(NNNN)", THPVariable_Wrap(std::get<0>(r)), THPVariable_Wrap(std::get<1>(r)),
                        THPVariable_Wrap(std::get<2>(r)), THPVariable_Wrap(std::get<3>(r)));
