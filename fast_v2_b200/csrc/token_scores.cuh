@@ -151,6 +151,21 @@ struct TokVec {  // 16 bytes of logits
   __device__ __forceinline__ static TokVec finite(uint4 u) {
     return TokVec(make_uint4(clamp_word<T>(u.x), clamp_word<T>(u.y), clamp_word<T>(u.z), clamp_word<T>(u.w)));
   }
+  // Entry e of a vector, and the entries not below x as bits.
+  __device__ __forceinline__ static float pick(uint4 u, int e) {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(e & 2 ? (e & 1 ? u.w : u.z) : (e & 1 ? u.y : u.x));
+    } else {
+      const float2 two = Pack2<T>::to(e & 4 ? (e & 2 ? u.w : u.z) : (e & 2 ? u.y : u.x));
+      return e & 1 ? two.y : two.x;
+    }
+  }
+  __device__ __forceinline__ unsigned reaching(float x) const {
+    unsigned bits = 0;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) bits |= !(f[e] < x) ? 1u << e : 0u;
+    return bits;
+  }
   __device__ __forceinline__ float max() const {
     float m = fmaxf(f[0], f[1]);
 #pragma unroll
@@ -464,6 +479,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
   if (a.top > 0) {
     for (;;) {
       const uint64_t tau = sh_tau;
+      const float tau_x = tau ? key_value(tau) : -INFINITY;
       auto offer = [&](float f, int idx) {
         const uint64_t k = score_key(f, idx);
         if (k >= tau) {
@@ -471,15 +487,24 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
           if (n < kTokList) sh_cand[n] = k;
         }
       };
-      auto offer_vector = [&](int i) {
-        const TokVec<T> q(*reinterpret_cast<const uint4*>(vec + static_cast<int64_t>(i) * 16));
-#pragma unroll
-        for (int e = 0; e < kN; ++e) offer(q.f[e], first + i * kN + e);
+      auto load_vector = [&](int i) { return *reinterpret_cast<const uint4*>(vec + static_cast<int64_t>(i) * 16); };
+      auto offer_vector = [&](uint4 u, int i) {
+        for (unsigned hits = TokVec<T>(u).reaching(tau_x); hits; hits &= hits - 1) {
+          const int e = __ffs(hits) - 1;
+          offer(TokVec<T>::pick(u, e), first + i * kN + e);
+        }
       };
       const bool in = threadIdx.x < nv && pass.most(first) >= tau;
       const bool more = in && pass.more(tau);
-      if (in && !more)
-        for (int i = pass.at; i <= pass.last(); i += NT) offer_vector(i);
+      if (in && !more) {
+        uint4 u[kTokUnroll];
+        const int last = pass.last();
+#pragma unroll
+        for (int j = 0; j < kTokUnroll; ++j) u[j] = load_vector(min(pass.at + j * NT, last));
+#pragma unroll
+        for (int j = 0; j < kTokUnroll; ++j)
+          if (pass.at + j * NT <= last) offer_vector(u[j], pass.at + j * NT);
+      }
       if (single >= 0) offer(lone, single);
       // the warp reads all vectors of such threads, all lanes at work
       const unsigned who = __ballot_sync(0xffffffffu, more);
@@ -489,7 +514,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
         int i = p;
         for (; i >= each; i -= each) w &= w - 1;
         i = warp * 32 + __ffs(w) - 1 + i * NT;
-        if (i < nv) offer_vector(i);
+        if (i < nv) offer_vector(load_vector(i), i);
       }
       __syncthreads();
       const int n = sh_n;
@@ -699,12 +724,10 @@ __global__ void __launch_bounds__(kTokRowWarps * 32, 4) token_scores_warp_kernel
     __syncwarp();
     const float tau_x = tau ? key_value(tau) : -INFINITY;
     auto offer = [&](float f, int idx) {
-      if (!(f < tau_x)) {
-        const uint64_t k = score_key(f, idx);
-        if (k >= tau) {
-          const int to = atomicAdd(count, 1);
-          if (to < kTokRowList) list[to] = k;
-        }
+      const uint64_t k = score_key(f, idx);
+      if (k >= tau) {
+        const int to = atomicAdd(count, 1);
+        if (to < kTokRowList) list[to] = k;
       }
     };
     // Which entries of four vectors at a time reach tau's value, as bits, and
@@ -717,10 +740,7 @@ __global__ void __launch_bounds__(kTokRowWarps * 32, 4) token_scores_warp_kernel
       unsigned hits = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const TokVec<T> q(u[j]);
-        unsigned some = 0;
-#pragma unroll
-        for (int e = 0; e < kN; ++e) some |= !(q.f[e] < tau_x) ? 1u << e : 0u;
+        const unsigned some = TokVec<T>(u[j]).reaching(tau_x);
         if (i0 + j * 32 < nv) hits |= some << (j * kN);
       }
       for (; hits; hits &= hits - 1) {
