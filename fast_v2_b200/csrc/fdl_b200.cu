@@ -83,18 +83,19 @@ PagedPlan paged_plan(int batch, int hq, int hkv, int head_dim, int64_t cap) {
   // with more units, one CTA of 4 warps each.  A cluster's time follows its
   // own sequence (0.7 us a tile and CTA), so a batch in which one sequence is
   // long waits for it; the line costs a scan and a second kernel, but shares
-  // any batch out evenly.  Measured on B200, 28 query / 4 KV heads of 128, all
-  // sequences of one length, cluster against line: 320 keys B=1 5.5 / 6.3 us,
-  // B=30 6.0 / 10.4 us; 1024 keys B=16 9.0 / 12.3 us; 4096 keys B=8 16.7 /
-  // 18.2 us; B=100 of 1 to 1024 keys 25.1 / 27.1 us, of 1 to 4096 keys 82.8 /
-  // 72.7 us.  The limits keep the worst case, one long sequence among short
-  // ones, at about twice the line's time.
+  // any batch out evenly and uses every SM.  Measured on B200, 28 query / 4 KV
+  // heads of 128, cluster against line: 320 keys B=1 5.4 / 6.0 us, B=30 6.0 /
+  // 10.2 us; 1024 keys B=16 9.0 / 10.9 us; 4096 keys B=8 16.4 / 20.2 us; 8192
+  // keys B=1 (32 CTAs) 12.2 / 10.5 us; B=100 of 1 to 1024 keys 22.7 / 27.0 us,
+  // of 1 to 4096 keys 76.7 / 72.6 us.  The limits keep the worst case, one long
+  // sequence among short ones, at about twice the line's time.
   const bool few = units <= 128 && head_dim <= 128;
   p.nw = few ? 8 : kPagedLineWarps;
   const int64_t tiles = (cap + p.nw * kPagedWarpKeys - 1) / (p.nw * kPagedWarpKeys);
   p.cluster = 1;
   while (p.cluster < 8 && units * p.cluster * 2 <= 128 && p.cluster < tiles) p.cluster *= 2;
-  if ((tiles + p.cluster - 1) / p.cluster > (few ? 8 : 16)) p.cluster = 0;
+  const int most = !few ? 16 : units * p.cluster > 64 ? 8 : 5;  // tiles of a CTA
+  if ((tiles + p.cluster - 1) / p.cluster > most) p.cluster = 0;
   if (p.cluster) {
     p.grid = static_cast<int>(units * p.cluster);
     return p;
@@ -950,25 +951,25 @@ int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int voc
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int64_t vectors = static_cast<int64_t>(vocab) * (dtype == FDL_F32 ? 4 : 2) / 16;
   // A warp a row for many short rows, half a CTA (128 threads) for many rows of
-  // middle length, else a CTA of 256, in a cluster where rows are few.
-  // Measured on B200, warp / half / whole, top 20: 70000 rows of 125 vectors
-  // 110 / 393 / 680 us, 8000 of 1062 50 / 85 / 117, 5000 of 1750 60 / 57 / 75,
-  // 2000 of 4000 64 / 44 / 47, 1500 of 12564 255 / 60 / 58.  With few rows the
-  // time is one row's: 100 of 625 vectors 8.8 (warp) against 8.0 us (cluster);
-  // a cluster of 8 pays for itself below two CTAs a SM (64 rows of 19008: 14.0
-  // us with 4, 18.6 with 8).
+  // middle length, else a CTA of 256.  Measured on B200, warp / half / whole,
+  // top 20: 70000 rows of 125 vectors 109 / 410 / 649 us, 800 of 625 9.0 / 10.6
+  // / 12.8, 8000 of 1062 50 / 70 / 98, 700 of 1250 14.4 / 12.3 / 13.2, 5000 of
+  // 1750 59 / 46 / 60, 2000 of 4000 64 / 37 / 40, 1300 of 6000 86 / 38 / 36, 1500
+  // of 12564 141 / 68 / 58.  A cluster of CTAs a row where rows are few and
+  // long: it costs 2 us (100 rows of 625 vectors 5.5 us without, 7.5 us with)
+  // and divides 0.6 us a thousand vectors (19008 vectors, 1 / 2 / 4 / 8 CTAs: 8
+  // rows 16.0 / 12.6 / 10.1 / 9.2 us, 64 rows 16.5 / 13.6 / 12.2 / 14.8 us).
   auto go = [&](auto t) -> int {
     using T = decltype(t);
     constexpr int kRing = kTokStages * kTokUnroll * kTokCta * 16;
     if (!smem_configured<token_scores_kernel<T, kTokCta>>(kRing)) return FDL_E_NODEVICE;
-    if (vectors <= 1280 && rows >= 4 * num_sms())
+    if (rows >= 4 * num_sms() && vectors <= (rows >= 16 * num_sms() ? 1280 : 640))
       return launch_after(token_scores_warp_kernel<T>, (rows + kTokRowWarps - 1) / kTokRowWarps, kTokRowWarps * 32, 0, s,
                           1, a);
-    if (vectors <= 6144 && rows >= 8 * num_sms())
+    if (rows >= 4 * num_sms() && vectors <= 5120)
       return launch_after(token_scores_kernel<T, kTokCta / 2>, rows, kTokCta / 2, kRing / 2, s, 1, a);
     int cluster = 1;
-    while (cluster < 8 && static_cast<int64_t>(rows) * cluster < 2ll * num_sms() && vectors >= 2ll * cluster * kTokCta)
-      cluster *= 2;
+    while (cluster < 8 && vectors >= 5000 && static_cast<int64_t>(rows) * cluster <= num_sms()) cluster *= 2;
     return launch_after(token_scores_kernel<T, kTokCta>, rows * cluster, kTokCta, kRing, s, cluster, a);
   };
   return dtype == FDL_BF16 ? go(__nv_bfloat16{}) : dtype == FDL_F16 ? go(__half{}) : go(float{});
