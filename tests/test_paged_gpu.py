@@ -284,6 +284,21 @@ def test_attention_shapes_of_batches(lens):
     _check_attn(*_attn_case(len(lens), lens, 28, 4, 128, 16, BF))
 
 
+@pytest.mark.parametrize("dt,page", [(BF, 16), (HF, 20)])
+@pytest.mark.parametrize("hq,hkv,D", [(28, 4, 128), (64, 4, 128), (33, 1, 128), (20, 1, 64), (64, 2, 64), (16, 1, 256),
+                                      (3, 3, 256)])
+def test_attention_on_one_line(hq, hkv, D, dt, page):
+    """Long caches: the tiles of all sequences are shared out over the GPU and
+    the pieces joined."""
+    _check_attn(*_attn_case(hq, [9000, 5, 0, 700, 64, 16389], hq, hkv, D, page, dt))
+
+
+def test_attention_on_one_line_with_many_sequences():
+    lens = [1] * 150 + [3000] + [0] * 50 + [64, 65, 1500] * 30 + [0]
+    _check_attn(*_attn_case(5, lens, 12, 2, 128, 16, BF))
+    _check_attn(*_attn_case(6, [0] * 290 + [2000], 12, 2, 128, 16, BF))
+
+
 def test_attention_peaked_and_flat_scores():
     for qs in (0.0, 30.0):
         q, k, v, table, lens = _attn_case(3, [700, 64, 1], 8, 2, 128, 16, BF, q_scale=qs)
