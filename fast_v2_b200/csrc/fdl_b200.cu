@@ -89,8 +89,13 @@ PagedPlan paged_plan(int batch, int hq, int hkv, int head_dim, int64_t cap) {
   // keys B=1 (32 CTAs) 12.2 / 10.5 us; B=100 of 1 to 1024 keys 22.7 / 27.0 us,
   // of 1 to 4096 keys 76.7 / 72.6 us.  The limits keep the worst case, one long
   // sequence among short ones, at about twice the line's time.
+  // Very many short units take fewer warps each, so that more of them run at
+  // once: 1140 units of up to 36 keys 8.3 / 6.3 / 5.6 us with 4 / 2 / 1 warps,
+  // 1000 of up to 16 keys 8.7 / 6.6 / 5.2, 600 of up to 60 5.9 / 4.6 / 5.4, 800 of
+  // up to 128 9.3 / 7.6 / 9.9, of up to 256 14.6 / 13.5 / 17.1.
   const bool few = units <= 128 && head_dim <= 128;
   p.nw = few ? 8 : kPagedLineWarps;
+  if (head_dim <= 128 && units > 2 * num_sms() && cap <= 256) p.nw = cap <= 48 ? 1 : 2;
   const int64_t tiles = (cap + p.nw * kPagedWarpKeys - 1) / (p.nw * kPagedWarpKeys);
   p.cluster = 1;
   while (p.cluster < 8 && units * p.cluster * 2 <= 128 && p.cluster < tiles) p.cluster *= 2;
@@ -902,17 +907,18 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_page
   auto go = [&](auto t, auto d, auto nh) -> int {
     using T = decltype(t);
     constexpr int D = decltype(d)::value, NH = decltype(nh)::value;
-    constexpr int smem4 = PagedCfg<D, 4, false>::kSmem, smem8 = PagedCfg<D, 8, false>::kSmem,
-                  smem_line = PagedCfg<D, 4, true>::kSmem;
-    if constexpr ((D) < 256)
-      if (plan.cluster && plan.nw == 8) {
-        if (!smem_configured<paged_attn_kernel<T, D, NH, 8, false>>(smem8)) return FDL_E_NODEVICE;
-        return launch_after(paged_attn_kernel<T, D, NH, 8, false>, plan.grid, 256, smem8, s, plan.cluster, a);
-      }
-    if (plan.cluster) {
-      if (!smem_configured<paged_attn_kernel<T, D, NH, 4, false>>(smem4)) return FDL_E_NODEVICE;
-      return launch_after(paged_attn_kernel<T, D, NH, 4, false>, plan.grid, 128, smem4, s, plan.cluster, a);
+    constexpr int smem_line = PagedCfg<D, 4, true>::kSmem;
+    auto apart = [&](auto warps) -> int {  // a unit a CTA or cluster
+      constexpr int NW = decltype(warps)::value, bytes = PagedCfg<D, NW, false>::kSmem;
+      if (!smem_configured<paged_attn_kernel<T, D, NH, NW, false>>(bytes)) return FDL_E_NODEVICE;
+      return launch_after(paged_attn_kernel<T, D, NH, NW, false>, plan.grid, NW * 32, bytes, s, plan.cluster, a);
+    };
+    if constexpr ((D) < 256) {
+      if (plan.cluster && plan.nw == 8) return apart(std::integral_constant<int, 8>{});
+      if (plan.cluster && plan.nw == 2) return apart(std::integral_constant<int, 2>{});
+      if (plan.cluster && plan.nw == 1) return apart(std::integral_constant<int, 1>{});
     }
+    if (plan.cluster) return apart(std::integral_constant<int, 4>{});
     if (!smem_configured<paged_attn_kernel<T, D, NH, 4, true>>(smem_line)) return FDL_E_NODEVICE;
     const int rc = launch_after(paged_attn_kernel<T, D, NH, 4, true>, plan.grid, 128, smem_line, s, 1, a);
     if (rc != FDL_OK) return rc;

@@ -21,9 +21,10 @@
 //            CTA, so it does not grow with the batch -- and a second kernel
 //            joins them in order.
 //   cluster  A thread-block cluster takes a unit, its CTAs equal parts of the
-//            unit's tiles, joined through distributed shared memory: one
-//            launch, no workspace.  For short caches, where the scan and the
-//            second kernel cost more than an uneven share.
+//            unit's tiles, joined through distributed shared memory -- or one
+//            CTA of 1 to 4 warps where units are many: one launch, no
+//            workspace.  For short caches, where the scan and the second
+//            kernel cost more than an uneven share.
 //
 // Within a CTA every warp takes 16 keys of a tile and runs on its own: its
 // rows arrive by cp.async in a ring of its own, no barrier between warps
@@ -78,7 +79,7 @@ constexpr float kPagedSlack = 8.f;
 // against 25.1 us).
 template <int D, int NW, bool LINE>
 struct PagedCfg {
-  static constexpr int kStages = D == 128 && !LINE && NW == 4 ? 2 : 3;
+  static constexpr int kStages = !LINE && (NW <= 2 || (NW == 4 && D == 128)) ? 2 : 3;
   static constexpr int kStage = 2 * kPagedWarpKeys * D * 2;  // bytes of a warp's tile: K rows, V rows
   static constexpr int kSmem = NW * kStages * kStage;
 };

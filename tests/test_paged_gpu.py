@@ -284,6 +284,16 @@ def test_attention_shapes_of_batches(lens):
     _check_attn(*_attn_case(len(lens), lens, 28, 4, 128, 16, BF))
 
 
+@pytest.mark.parametrize("hq,hkv,D", [(28, 4, 128), (64, 4, 128), (16, 16, 64), (64, 2, 64), (6, 6, 256)])
+@pytest.mark.parametrize("most", [30, 45, 48, 49, 100, 256, 257])
+@pytest.mark.parametrize("page", [16, 5])
+def test_attention_of_many_short_sequences(hq, hkv, D, most, page):
+    lens = [i * 37 % (most + 1) for i in range(330 // hkv * 4 // min(4, hkv) + 300 // hkv)]
+    lens[0], lens[1] = most, 0
+    q, k, v, table, n = _attn_case(most, lens, hq, hkv, D, page, HF if most % 2 else BF)
+    _check_attn(q, k, v, table[:, : R.pages_of(most, page)], n)
+
+
 @pytest.mark.parametrize("dt,page", [(BF, 16), (HF, 20)])
 @pytest.mark.parametrize("hq,hkv,D", [(28, 4, 128), (64, 4, 128), (33, 1, 128), (20, 1, 64), (64, 2, 64), (16, 1, 256),
                                       (3, 3, 256)])
