@@ -101,6 +101,9 @@ PagedPlan paged_plan(int batch, int hq, int hkv, int head_dim, int64_t cap) {
   while (p.cluster < 8 && units * p.cluster * 2 <= 128 && p.cluster < tiles) p.cluster *= 2;
   const int most = !few ? 16 : units * p.cluster > 64 ? 8 : 5;  // tiles of a CTA
   if ((tiles + p.cluster - 1) / p.cluster > most) p.cluster = 0;
+  // Two CTAs of 4 warps a unit while three CTAs a SM hold them all (160 units of
+  // up to 1000 keys 13.8 against 16.7 us; 240 units 17.6 / 17.5).
+  if (p.cluster == 1 && p.nw == 4 && head_dim <= 128 && tiles >= 8 && 2 * units <= 3 * num_sms()) p.cluster = 2;
   if (p.cluster) {
     p.grid = static_cast<int>(units * p.cluster);
     return p;

@@ -279,7 +279,8 @@ def test_attention_pages(page, layout):
 
 
 @pytest.mark.parametrize("lens", [[1], [0], [2], [31], [5000], [40001], [0, 0, 0], [1] * 300, [130] * 40,
-                                  [20000, 1, 1, 1, 3, 0, 9000], list(range(150))])
+                                  [20000, 1, 1, 1, 3, 0, 9000], list(range(150)),
+                                  [1000, 1, 0, 63, 64, 65, 129, 1023] * 5])
 def test_attention_shapes_of_batches(lens):
     _check_attn(*_attn_case(len(lens), lens, 28, 4, 128, 16, BF))
 
