@@ -387,17 +387,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
   if (rank == 0 && threadIdx.x < head) single = threadIdx.x;
   if (rank == ranks - 1 && threadIdx.x >= 32 && threadIdx.x - 32 < rest) single = a.V - rest + threadIdx.x - 32;
 
-  // the target's logit is on its way from the start
-  int64_t target = -1;
-  float target_x = 0.f;
-  if (rank == 0 && threadIdx.x == 0) {
-    target = a.targets[row];
-    if (target >= 0 && target < a.V) target_x = static_cast<float>(x[target]);
-  }
+  // the target is read during the pass, its logit behind it
+  const int64_t target = rank == 0 && threadIdx.x == 0 ? a.targets[row] : -1;
 
   // ---- the one pass
   TokPass<T, NT> pass;
   pass.run_ring(vec, nv, threadIdx.x, ring);
+  const float target_x = target >= 0 && target < a.V ? static_cast<float>(x[target]) : 0.f;
   TokSums s = pass.sums.natural();
   float lone = -INFINITY;
   if (single >= 0) {
