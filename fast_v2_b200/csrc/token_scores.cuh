@@ -22,16 +22,17 @@
 // lower index first).  If there are k threads whose largest entry is at or
 // above tau, then at least k entries are, so every one of the top k is -- and
 // lies with a thread whose largest entry is at or above tau.  In a CTA tau is
-// the k-th largest of the r = ceil(k / W) largest thread maxima of each of W
-// warps, in a warp the k-th largest lane maximum; only the vectors of the
+// the k-th largest of the r = ceil(1.5 k / W) largest thread maxima of each of W
+// warps (r = ceil(k / W) leaves more to rank: 512 rows, top 32, 49 us against
+// 40), in a warp the k-th largest lane maximum; only the vectors of the
 // threads at or above it are read again (k and a few, from L2 or L1), the
 // entries at or above tau are collected and put in order.  Rows with very many
 // entries above tau (long runs of equal logits, say) overflow the list; the
 // k-th best of the entries caught is then a better tau.
 //
-// Measured: 512 rows of 152064 bf16 logits, top 20, 39 us (4.0 TB/s; 34 us
-// without the top), 1500 rows of 50257 fp32, top 5, 53 us (5.7 TB/s), 8 rows of
-// 152064 9.2 us.
+// Measured: 512 rows of 152064 bf16 logits, top 20, 38 us (4.1 TB/s; 34 us
+// without the top), 1500 rows of 50257 fp32, top 5, 52 us (5.8 TB/s), 8 rows of
+// 152064 9.0 us.
 #pragma once
 #include <type_traits>
 
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
   constexpr int kN = TokVec<T>::kN, kWarps = NT / 32;
   extern __shared__ __align__(16) char ring[];
   __shared__ float sh_m[kWarps], sh_z[kWarps], sh_t[kWarps];
-  __shared__ uint64_t sh_max[kWarps + kTokMaxTop];  // the largest thread maxima of each warp
+  __shared__ uint64_t sh_max[kWarps + kTokMaxTop * 3 / 2];  // the largest thread maxima of each warp
   __shared__ uint64_t sh_tau;
   __shared__ __align__(16) uint64_t sh_cand[kTokList];
   __shared__ uint64_t sh_top[kTokMaxTop];
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_scores_kernel(const __gri
   if (lane == 0) sh_m[warp] = m;
   // the r largest thread maxima of each warp
   const int full = min(nv / 32, kWarps);  // warps with a vector for every thread
-  const int r = full > 0 ? (a.top + full - 1) / full : 0;
+  const int r = full > 0 ? min(32, (a.top * 3 / 2 + full - 1) / full) : 0;
   if (warp < full) {
     uint32_t order = pass.least_order();
     const uint32_t index = pass.least_index(first);
