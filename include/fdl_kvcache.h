@@ -486,7 +486,8 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
  * over keys j < lens[b] (clamped to the table's width, FDL_DEV_LENGTH).  q and
  * out [B, hq, D] with strides; bf16 or f16, D 64, 128 or 256, hq <= 4096, any
  * hq / hkv.  A sequence without keys gives zeros.  A page outside [0, num_pages) hides its keys and
- * is reported.  Softmax in fp32.  workspace: at least
+ * is reported.  Softmax in fp32; a weight enters the product as two numbers of
+ * V's type.  workspace: at least
  * fdl_paged_attn_workspace_bytes() bytes, 16-byte aligned, not shared with a
  * call that may run at the same time; its contents need not be kept.
  * ---------------------------------------------------------------------- */

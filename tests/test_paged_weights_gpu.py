@@ -1,0 +1,83 @@
+"""GPU tests of the accuracy of one-token attention's softmax weights: what a
+16-bit product could lose of them."""
+import pytest
+import torch
+
+from fast_v2_b200 import _lib, paged
+from tests import _paged_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def _ops():
+    _lib.ensure_ops()
+    _lib.last_device_error()
+    yield
+    code, info = _lib.last_device_error()
+    assert code == 0, f"device error {code} (info {info}) left by the test"
+
+
+def _dense(q, k, v, lens, scale):
+    """(out, bound) in 64 bits over K and V [B, n, hkv, D].  bound: half a step
+    of the output; a weight goes into the product as two numbers of V's type,
+    which leaves h^2 of it; D + 4 roundings of a score of magnitude sum |q k|
+    move a weight by that much relative, in the numerator and in the sum; 200
+    fp32 roundings of sums and joins.  fp16 alone: what is below 2^-14 is a
+    multiple of 2^-24, next to a largest weight of 2^-5 in each 16 keys: 2^-20
+    a key, 2^-16 of the largest value."""
+    B, hq, D = q.shape
+    h, u = R.half_step(q.dtype), R.U32
+    out = torch.zeros(B, hq, D, dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        kk, vv = (t[b, :n].double().repeat_interleave(hq // t.shape[2], 1).transpose(0, 1) for t in (k, v))
+        qq = q[b].double()[:, None]
+        p = torch.softmax((qq @ kk.transpose(1, 2))[:, 0] * scale, -1)
+        out[b] = (p[:, None] @ vv)[:, 0]
+        mass = (p[:, None] @ vv.abs())[:, 0]
+        ds = (qq.abs() @ kk.abs().transpose(1, 2)).amax((1, 2)) * abs(scale) * (D + 4) * u
+        bound[b] = h * out[b].abs() + (h * h + 2 * ds[:, None] + 200 * u) * mass * (1 + h)
+        if q.dtype == HF:
+            bound[b] += 2.0 ** -16 * vv.abs().amax((0, 1)) + 2.0 ** -24
+    return out, bound
+
+
+def _paged(k, v, page):
+    """Dense K and V [B, n, hkv, D] as pages in reverse order and their table."""
+    B, n, hkv, D = k.shape
+    each = R.pages_of(n, page)
+    pool = []
+    for t in (k, v):
+        full = torch.zeros(B, each * page, hkv, D, dtype=t.dtype, device=DEV)
+        full[:, :n] = t
+        pool.append(full.view(B * each, page, hkv, D).flip(0).contiguous())
+    table = torch.arange(B * each - 1, -1, -1, device=DEV, dtype=torch.int32).view(B, each)
+    return pool[0], pool[1], table
+
+
+def _check(q, k, v, lens, scale, page=16):
+    kp, vp, table = _paged(k, v, page)
+    out = paged.decode_attention(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device=DEV), scale)
+    ref, bound = _dense(q, k, v, lens, scale)
+    R.assert_within("attention", out, ref, bound)
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(28, 4, 128), (64, 4, 128), (16, 16, 64), (6, 2, 256)])
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("most", [40, 900, 9000])
+def test_weights_are_not_cut_to_16_bits(most, dt, hq, hkv, D):
+    """Values that nearly cancel show a weight's rounding; few keys do not
+    average it out."""
+    g = torch.Generator(device=DEV).manual_seed(most + D)
+    lens = [2, 3, 5, 0, 17, 33, most]
+    B = len(lens)
+    k, v = (torch.randn(B, most, hkv, D, generator=g, device=DEV).to(dt) for _ in range(2))
+    sign = torch.where(torch.arange(most, device=DEV) % 2 == 0, 1.0, -1.0)[None, :, None, None]
+    v = (sign * (1 + v.abs().float() / 8)).to(dt)
+    q = (2 * torch.randn(B, hq, D, generator=g, device=DEV)).to(dt)
+    _check(q, k, v, lens, D ** -0.5)
