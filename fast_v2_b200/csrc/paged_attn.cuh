@@ -69,8 +69,18 @@ constexpr int kPagedWarpKeys = 16;
 constexpr int kPagedLineWarps = 4;
 constexpr int kPagedLineTile = kPagedLineWarps * kPagedWarpKeys;
 // A score may pass the running reference by 2^8 before the sums are scaled
-// down to a new one (p <= 256 in either 16-bit type).
+// down to a new one.
 constexpr float kPagedSlack = 8.f;
+// fp16 has no numbers below 2^-24.  Its weights are lifted by 2^7 (p <= 2^15),
+// which cancels in the quotient: a key behind a strong one loses at most 2^-32
+// of the strong one's weight, 2^-24 for the 256 keys that a warp takes in the
+// forms for short caches.  On the line it may take 2^15 and more.  There the
+// reference also moves down, to the largest score of a tile that lies 2^12
+// below it, and the weak keys keep their share; down to 2^40 below the largest
+// score at most, so that the sums stay inside fp32.
+constexpr float kPagedLift = 7.f;
+constexpr float kPagedFar = 12.f;
+constexpr float kPagedDepth = 40.f;
 
 // Stages of a warp's ring.  On the line two CTAs a SM (D = 128) with three
 // stages keep HBM busy (30.7 us for 65k keys against 31.7 us with three CTAs
@@ -152,6 +162,7 @@ template <typename T, int D, int NH, int NW, bool LINE>
 __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   using Cfg = PagedCfg<D, NW, LINE>;
   constexpr int kThreads = NW * 32, kTile = NW * kPagedWarpKeys;
+  constexpr bool kNarrow = std::is_same<T, __half>::value, kFollow = kNarrow && LINE;
   constexpr int kStages = Cfg::kStages, kChunks = D / 8, kRowB = D * 2, H = 8 * NH;
   constexpr int kLoads = kPagedWarpKeys * kChunks / 32;  // 16-byte pieces of K (and of V) a lane and tile
   extern __shared__ __align__(128) char smem[];
@@ -349,6 +360,7 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
   uint32_t qf[NH][D / 16][2];
   float o[NH][D / 16][4];
   float m[NH][2], l[NH][2];
+  float deep[NH][2];  // kFollow: how far down the reference may move
   auto load_q = [&]() {  // the query heads of p's unit
     const int h0 = p.kh * a.G + p.hg * H, hn = min(H, a.G - p.hg * H);
     const T* q = static_cast<const T*>(a.q) + p.b * a.q_sb + h0 * a.q_sh;
@@ -369,7 +381,7 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
       for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[x][kk][e] = 0.f;
-      m[x][0] = m[x][1] = -INFINITY;
+      m[x][0] = m[x][1] = deep[x][0] = deep[x][1] = -INFINITY;
       l[x][0] = l[x][1] = 0.f;
     }
   };
@@ -456,7 +468,7 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
       }
       uint32_t pf[NH][2], pl[NH][2];
       float v[NH][4];  // keys g, g, g + 8, g + 8 of heads 2 c4, 2 c4 + 1
-      bool above = false;
+      bool above = false, near = true;
 #pragma unroll
       for (int x = 0; x < NH; ++x) {
 #pragma unroll
@@ -467,8 +479,16 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
         }
         const float t0 = fmaxf(v[x][0], v[x][2]), t1 = fmaxf(v[x][1], v[x][3]);
         above = above || t0 > m[x][0] + kPagedSlack || t1 > m[x][1] + kPagedSlack;
+        near = near && t0 >= m[x][0] - kPagedFar && t1 >= m[x][1] - kPagedFar;
       }
-      if (__any_sync(0xffffffffu, above)) {
+      bool move = __any_sync(0xffffffffu, above);
+      if constexpr (kFollow) {  // a lane's heads have to be near in one of the eight lanes that share them
+        unsigned all = __ballot_sync(0xffffffffu, near);
+        all |= all >> 16;
+        all |= all >> 8;
+        move = move || ((all | all >> 4) & 0xfu) != 0xfu;
+      }
+      if (move) {
 #pragma unroll
         for (int x = 0; x < NH; ++x) {
           float t0 = fmaxf(v[x][0], v[x][2]), t1 = fmaxf(v[x][1], v[x][3]);
@@ -477,7 +497,13 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
             t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
           }
-          const float n0 = fmaxf(m[x][0], t0), n1 = fmaxf(m[x][1], t1);
+          float n0 = fmaxf(m[x][0], t0), n1 = fmaxf(m[x][1], t1);
+          if constexpr (kFollow) {
+            deep[x][0] = fmaxf(deep[x][0], n0 - kPagedDepth);
+            deep[x][1] = fmaxf(deep[x][1], n1 - kPagedDepth);
+            if (t0 < m[x][0] - kPagedFar && t0 != -INFINITY) n0 = fminf(n0, fmaxf(t0, deep[x][0]));
+            if (t1 < m[x][1] - kPagedFar && t1 != -INFINITY) n1 = fminf(n1, fmaxf(t1, deep[x][1]));
+          }
           const float f0 = n0 == -INFINITY ? 1.f : ex2(m[x][0] - n0), f1 = n1 == -INFINITY ? 1.f : ex2(m[x][1] - n1);
           m[x][0] = n0;
           m[x][1] = n1;
@@ -494,7 +520,8 @@ __global__ void __launch_bounds__(NW * 32) paged_attn_kernel(const __grid_consta
       }
 #pragma unroll
       for (int x = 0; x < NH; ++x) {
-        const float r0 = m[x][0] == -INFINITY ? 0.f : m[x][0], r1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
+        constexpr float lift = kNarrow ? kPagedLift : 0.f;
+        const float r0 = (m[x][0] == -INFINITY ? 0.f : m[x][0]) - lift, r1 = (m[x][1] == -INFINITY ? 0.f : m[x][1]) - lift;
         // A weight goes into the product as two numbers of V's type, its
         // rounded value and what that leaves: 2^-16 (bf16) or 2^-22 (fp16) of
         // it is lost.  One number would lose 2^-8 or 2^-11, as much as the

@@ -1,5 +1,7 @@
 """GPU tests of the accuracy of one-token attention's softmax weights: what a
-16-bit product could lose of them."""
+16-bit product could lose of them, and what one strong key could hide."""
+import math
+
 import pytest
 import torch
 
@@ -81,3 +83,68 @@ def test_weights_are_not_cut_to_16_bits(most, dt, hq, hkv, D):
     v = (sign * (1 + v.abs().float() / 8)).to(dt)
     q = (2 * torch.randn(B, hq, D, generator=g, device=DEV)).to(dt)
     _check(q, k, v, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("lead", [8.0, 11.0, 16.0, 17.4, 25.0])
+@pytest.mark.parametrize("B,n,where", [(1, 131072, "first"), (1, 131072, "last"), (6, 40000, "middle"), (8, 3000, "first"),
+                                       (2, 250, "last"), (200, 400, "first")])
+def test_weak_keys_behind_a_strong_one_keep_their_share(B, n, where, lead, dt):
+    """One key leads all others, which are equal, by `lead` nats: their share
+    is (n - 1) / (n - 1 + e^lead) whatever their place, on the line and in the
+    forms for short caches."""
+    D, hq, hkv = 64, 4, 2
+    at = {"first": 0, "middle": n // 2 + 5, "last": n - 1}[where]
+    k = torch.zeros(B, n, hkv, D, dtype=dt, device=DEV)
+    k[:, at, :, 0] = 8.0
+    v = torch.zeros(B, n, hkv, D, dtype=dt, device=DEV)
+    v[:] = torch.linspace(0.5, 8, D, device=DEV).to(dt)
+    v[:, at] = 0
+    q = torch.zeros(B, hq, D, dtype=dt, device=DEV)
+    q[:, :, 0] = 1.0
+    scale = lead / 8.0
+    _check(q, k, v, [n] * B, scale)
+    v[:, at] = -2.0
+    _check(q, k, v, [n - 1 if where == "middle" else n] * B, scale)
+
+
+@pytest.mark.parametrize("lead", [14.0, 17.0, 17.4, 22.0])
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (24, 2)])
+def test_many_weak_keys_of_one_warp_keep_their_share(hq, hkv, dt, lead):
+    """With many sequences a warp walks tens of thousands of keys behind the
+    strong one (the sequences share their pages)."""
+    B, n, D = 150, 131072, 64
+    k = torch.zeros(1, n, hkv, D, dtype=dt, device=DEV)
+    k[:, 0, :, 0] = 8.0
+    k[:, 60000, :, 0] = 4.0  # and another one on the way
+    v = torch.zeros(1, n, hkv, D, dtype=dt, device=DEV)
+    v[:] = torch.linspace(0.5, 8, D, device=DEV).to(dt)
+    v[:, 0] = 0
+    q = torch.zeros(B, hq, D, dtype=dt, device=DEV)
+    q[:, :, 0] = 1.0
+    q[:, 1::2, 0] = 0.0  # every second head weighs all keys alike
+    kp, vp, table = _paged(k, v, 16)
+    out = paged.decode_attention(q, kp, vp, table.repeat(B, 1), torch.full((B,), n, dtype=torch.int32, device=DEV),
+                                 lead / 8.0)
+    ref, bound = _dense(q[:1], k, v, [n], lead / 8.0)
+    R.assert_within("attention", out, ref.expand(B, hq, D), bound.expand(B, hq, D))
+
+
+def test_tiles_far_below_the_reference_with_infinite_scores_and_masked_pages():
+    D = 64
+    k = torch.zeros(1, 400, 1, D, dtype=HF, device=DEV)
+    v = torch.ones(1, 400, 1, D, dtype=HF, device=DEV)
+    k[0, 3, 0, 0] = 40.0
+    k[0, 64:192, 0, 1] = -math.inf  # tiles without a finite score
+    q = torch.zeros(1, 8, D, dtype=HF, device=DEV)
+    q[:, :, 0] = 1.0
+    q[:, :, 1] = 1.0
+    kp, vp, table = _paged(k, v, 16)
+    lens = torch.tensor([400], dtype=torch.int32, device=DEV)
+    out = paged.decode_attention(q, kp, vp, table, lens, 1.0)
+    assert bool((out == 1).all())
+    table[0, 13] = -1  # and a tile without a page
+    out = paged.decode_attention(q, kp, vp, table, lens, 1.0)
+    assert _lib.last_device_error() == (1, -1)
+    assert bool((out == 1).all())
