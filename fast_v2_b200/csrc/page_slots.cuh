@@ -171,7 +171,10 @@ __global__ void __launch_bounds__(kSlotsThreads) page_slots_kernel(const __grid_
     const int len = a.lens[b];
     a.new_lens[b] = s_at[b] >= 0 ? len + a.n_new[b] : len;
   }
-  if (threadIdx.x == 0) a.new_count[0] = count - sh_taken;
+  if (threadIdx.x == 0) {
+    a.new_count[0] = count - sh_taken;
+    a.new_count[1] = 0;  // the ticket of a call that takes it as its count
+  }
 }
 
 // Pages of finished sequences go back on the stack, in the order of the rows

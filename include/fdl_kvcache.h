@@ -453,8 +453,8 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
  * A sequence's new pages come off the end of free_pages[0 .. count[0]) (a
  * stack; n_free is its capacity), in the order of the sequences, and are
  * written into its table row behind the ceil(lens[b] / page_size) it has.
- * new_lens[b] = lens[b] + n_new[b], new_count[0] = the pages left; both may be
- * the inputs themselves (in place).  count is int32[2]: count[1] is scratch,
+ * new_lens[b] = lens[b] + n_new[b], new_count = {the pages left, 0}; both may
+ * be the inputs themselves (in place).  count is int32[2]: count[1] is scratch,
  * 0 before and after a call, so calls on one count must not overlap.  A
  * request that cannot be served (a negative length, no room in its table row,
  * pages or rows that run out) is refused whole: slots -1, length unchanged, no
