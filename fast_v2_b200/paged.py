@@ -52,9 +52,10 @@ def build_slots(lens, n_new, block_table, free_pages, free_count, page_size: int
     Writes slots, positions int64 [rows] (-1 and 0 behind the last token),
     cu_seqlens int32 [B + 1], and the new lengths and free count to
     new_lens [B] and new_count [2] (no values needed before), in place on lens
-    and free_count where not given.  A sequence that cannot be served (no page, no room in its table
-    row or in ``slots``) is refused whole and reported in the device status:
-    slots -1, its length unchanged.
+    and free_count where not given.  A sequence that cannot be served (no free
+    page, no room in its table row or in ``slots``, no table entry for the page
+    it has begun) is refused whole and reported in the device status: slots -1,
+    its length unchanged.
     """
     _call("page_slots", lens, n_new, block_table, free_pages, free_count, page_size, slots, positions, cu_seqlens,
           new_lens, new_count)

@@ -457,9 +457,11 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
  * be the inputs themselves (in place).  count is int32[2]: count[1] is scratch,
  * 0 before and after a call, so calls on one count must not overlap.  A
  * request that cannot be served (a negative length, no room in its table row,
- * pages or rows that run out) is refused whole: slots -1, length unchanged, no
- * page taken, FDL_DEV_LENGTH (info = b); sequences behind it that need pages
- * are refused with it when the pool is what ran out.  Rows behind the last
+ * no entry for the page that its first token goes into, pages or rows that run
+ * out) is refused whole: slots -1, length unchanged, no page taken,
+ * FDL_DEV_LENGTH (info = b); sequences behind it that need pages are refused
+ * with it when the pool is what ran out.  A negative page on the stack gives
+ * slots of -1 and FDL_DEV_INDEX (info = page).  Rows behind the last
  * token get slot -1 and position 0.  batch <= 4096, (max_pages + 1) *
  * page_size < 2^31.
  *
