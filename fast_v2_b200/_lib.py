@@ -118,6 +118,13 @@ def ensure_ops() -> None:
         _ops_loaded = True
 
 
+def load_if_built() -> None:
+    """ensure_ops() where the libraries are there, for modules whose functions
+    may be traced: a compiler that meets torch.ops.fdl first cannot load it."""
+    if LIB_ABI.exists() and LIB_TORCH.exists():
+        ensure_ops()
+
+
 def direct():
     """The native module whose functions take plain CUDA tensors straight into
     the operators of torch.ops.fdl, or return NotImplemented where the call has

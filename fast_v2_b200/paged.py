@@ -30,6 +30,8 @@ from . import _lib
 
 MAX_BATCH = 4096
 
+_lib.load_if_built()
+
 
 def _call(name: str, *args) -> None:
     """An operator without a result: straight into the library for plain CUDA

@@ -18,6 +18,8 @@ from . import _lib
 
 MAX_TOP = 32
 
+_lib.load_if_built()
+
 
 class TokenScores(NamedTuple):
     logprob: torch.Tensor                 # fp32 [rows]

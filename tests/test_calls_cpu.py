@@ -1,0 +1,40 @@
+"""CPU checks of the ways into the operators: compiled calls, hosts without
+Python, calls under modes and traces."""
+import subprocess
+import sys
+from pathlib import Path
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def _fresh(program: str) -> str:
+    r = subprocess.run([sys.executable, "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-4000:]
+    return r.stdout
+
+
+COMPILED = {
+    "scores": "scoring.token_logprobs(torch.empty(9, 1000, device='meta'), e(9, torch.int64), 3).top_token",
+    "attention": "paged.decode_attention(h(2, 8, 64), h(4, 16, 2, 64), h(4, 16, 2, 64), e((2, 3)), e(2))",
+    "slots": "paged.build_slots(e(2), e(2), e((2, 3)), e(9), e(2), 16, e(5, torch.int64), e(5, torch.int64), e(3))",
+    "rope": "paged.norm_rope_store(h(5, 12 * 64), e(5, torch.int64), e(16, torch.float32), h(5, 8, 64), "
+            "h(4, 16, 2, 64), h(4, 16, 2, 64), e(5, torch.int64))",
+    "release": "paged.release_pages(e(2, torch.bool), e(2), e((2, 3)), e(9), e(2), 16)",
+}
+
+
+def test_the_first_call_of_a_process_may_be_compiled():
+    calls = ", ".join(f"lambda: {c}" for c in COMPILED.values())
+    out = _fresh(f"""
+import torch
+from fast_v2_b200 import paged, scoring
+def e(n, t=torch.int32): return torch.empty(n, dtype=t, device='meta')
+def h(*n): return torch.empty(n, dtype=torch.bfloat16, device='meta')
+for call in ({calls}):
+    def f(x):
+        r = call()
+        return (r if r is not None else x) + 1
+    print(tuple(torch.compile(f, fullgraph=True, backend='eager')(torch.empty(7, device='meta')).shape))
+    torch._dynamo.reset()
+""")
+    assert out.split("\n")[-6:-1] == ["(9, 3)", "(2, 8, 64)", "(7,)", "(7,)", "(7,)"]
