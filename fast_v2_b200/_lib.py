@@ -2,7 +2,8 @@
 
 ``abi()`` returns a :class:`ctypes.CDLL` for ``libfdl_b200.so`` (the C ABI of
 ``include/fdl_kvcache.h``); ``ensure_ops()`` registers the ``torch.ops.fdl``
-operators from ``libfdl_torch.so``.  There is no fallback: if a library is
+operators from ``libfdl_torch.so``; ``direct()`` is the Python module
+``libfdl_direct.so``, which calls some of them.  There is no fallback: if a library is
 missing or fails to load, an ``ImportError`` names the file and the command
 that builds it.
 """
@@ -17,6 +18,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_ABI = PKG / "libfdl_b200.so"
 LIB_TORCH = PKG / "libfdl_torch.so"
+LIB_DIRECT = PKG / "libfdl_direct.so"
 
 # Every symbol declared in include/fdl_kvcache.h.
 EXPORTS = (
@@ -98,7 +100,7 @@ def abi() -> ctypes.CDLL:
 
 def ensure_ops() -> None:
     """Register torch.ops.fdl.* (idempotent)."""
-    global _ops_loaded, _direct
+    global _ops_loaded
     if _ops_loaded:
         return
     abi()  # libfdl_torch.so resolves its C-ABI symbols from the loaded library
@@ -110,11 +112,6 @@ def ensure_ops() -> None:
         import torch
 
         torch.ops.load_library(str(LIB_TORCH))
-        # The same library as a Python module: its operators for plain CUDA
-        # tensors without the dispatcher (see direct()).
-        loader = importlib.machinery.ExtensionFileLoader(LIB_TORCH.stem, str(LIB_TORCH))
-        spec = importlib.util.spec_from_loader(LIB_TORCH.stem, loader)
-        _direct = importlib.util.module_from_spec(spec)
         _ops_loaded = True
 
 
@@ -129,8 +126,15 @@ def direct():
     """The native module whose functions take plain CUDA tensors straight into
     the operators of torch.ops.fdl, or return NotImplemented where the call has
     to go through the dispatcher (tensor subclasses, dispatch modes)."""
+    global _direct
     if _direct is None:
-        ensure_ops()
+        ensure_ops()  # libfdl_direct.so resolves its operators from libfdl_torch.so
+        with _lock:
+            if _direct is None:
+                if not LIB_DIRECT.exists():
+                    raise _missing(LIB_DIRECT)
+                loader = importlib.machinery.ExtensionFileLoader(LIB_DIRECT.stem, str(LIB_DIRECT))
+                _direct = importlib.util.module_from_spec(importlib.util.spec_from_loader(LIB_DIRECT.stem, loader))
     return _direct
 
 

@@ -1,13 +1,15 @@
-"""Build the two in-tree shared libraries of the package.
+"""Build the three in-tree shared libraries of the package.
 
 * ``libfdl_b200.so``  -- the C ABI of ``include/fdl_kvcache.h`` (all CUDA
   kernels), compiled by nvcc for sm_100a only.  Depends on the CUDA runtime
   alone; no torch types cross this boundary.
 * ``libfdl_torch.so`` -- ``torch.library`` registration of the ``fdl`` ops on
   top of that ABI (host C++ only), linked against ``libfdl_b200.so`` with an
-  ``$ORIGIN`` rpath.
+  ``$ORIGIN`` rpath.  Needs libtorch, not Python.
+* ``libfdl_direct.so`` -- the Python module that calls some of these operators
+  without the dispatcher, linked against ``libfdl_torch.so``.
 
-Both land next to this file so they travel with the source tree.  Run as
+They land next to this file so they travel with the source tree.  Run as
 ``python -m fast_v2_b200.build`` or call :func:`build`.
 """
 from __future__ import annotations
@@ -24,6 +26,7 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB_ABI = PKG / "libfdl_b200.so"
 LIB_TORCH = PKG / "libfdl_torch.so"
+LIB_DIRECT = PKG / "libfdl_direct.so"
 
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -65,33 +68,41 @@ def build_abi(force: bool = False, verbose: bool = False, ptxas_verbose: bool = 
     return LIB_ABI
 
 
-def build_torch(force: bool = False, verbose: bool = False) -> Path:
-    deps = [CSRC / "torch_ops.cpp", INCLUDE / "fdl_kvcache.h", LIB_ABI]
-    if not force and not _stale(LIB_TORCH, deps):
-        return LIB_TORCH
+def _build_host(source: str, target: Path, libs: list[str], incs: list[str], verbose: bool) -> None:
     import torch
     from torch.utils import cpp_extension as ce
 
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    incs = ce.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"]]
-    libdirs = ce.library_paths(device_type="cuda")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", str(CSRC / "torch_ops.cpp"), "-o", str(LIB_TORCH) + ".tmp"]
-    cmd += [f"-I{d}" for d in incs]
-    cmd += [f"-L{d}" for d in libdirs]
-    cmd += [f"-L{PKG}", "-lfdl_b200", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-            "-ltorch_cuda", "-ltorch_python", "-lcudart"]
+           "-DTORCH_API_INCLUDE_EXTENSION_H", str(CSRC / source), "-o", str(target) + ".tmp"]
+    cmd += [f"-I{d}" for d in ce.include_paths(device_type="cuda") + incs]
+    cmd += [f"-L{d}" for d in ce.library_paths(device_type="cuda")]
+    cmd += [f"-L{PKG}", *libs, "-Wl,-rpath,$ORIGIN"]
     _run(cmd, verbose)
-    os.replace(str(LIB_TORCH) + ".tmp", LIB_TORCH)
+    os.replace(str(target) + ".tmp", target)
+
+
+def build_torch(force: bool = False, verbose: bool = False) -> Path:
+    deps = [CSRC / "torch_ops.cpp", CSRC / "torch_ops.h", INCLUDE / "fdl_kvcache.h", LIB_ABI]
+    if force or _stale(LIB_TORCH, deps):
+        _build_host("torch_ops.cpp", LIB_TORCH, ["-lfdl_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+                                                 "-ltorch_cuda", "-lcudart"], [], verbose)
     return LIB_TORCH
 
 
-def build(force: bool = False, verbose: bool = False) -> tuple[Path, Path]:
-    return build_abi(force, verbose), build_torch(force, verbose)
+def build_direct(force: bool = False, verbose: bool = False) -> Path:
+    deps = [CSRC / "torch_direct.cpp", CSRC / "torch_ops.h", LIB_TORCH]
+    if force or _stale(LIB_DIRECT, deps):
+        _build_host("torch_direct.cpp", LIB_DIRECT, ["-lfdl_torch", "-lfdl_b200", "-lc10", "-ltorch", "-ltorch_cpu",
+                                                     "-ltorch_python"], [sysconfig.get_paths()["include"]], verbose)
+    return LIB_DIRECT
+
+
+def build(force: bool = False, verbose: bool = False) -> tuple[Path, Path, Path]:
+    return build_abi(force, verbose), build_torch(force, verbose), build_direct(force, verbose)
 
 
 if __name__ == "__main__":
     force = "--force" in sys.argv
-    a, t = build(force=force, verbose="-v" in sys.argv)
-    print(a)
-    print(t)
+    for lib in build(force=force, verbose="-v" in sys.argv):
+        print(lib)

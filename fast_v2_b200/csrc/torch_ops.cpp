@@ -5,20 +5,16 @@
 // implementation so torch.compile(fullgraph=True) and CUDA-graph capture can
 // trace through it -- the same contract as the custom-op wrapper around
 // flash_attn_with_kvcache in utils/attention_backends.py:73-120.
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
-#include <tuple>
 #include <vector>
 
 #include "../../include/fdl_kvcache.h"
+#include "torch_ops.h"
 
 namespace {
 
@@ -662,7 +658,9 @@ void check_pool(const Tensor& lens, const Tensor& free_pages, const Tensor& free
   check_i32(free_count, lens, 2, "free_count");
 }
 
-void page_slots(const Tensor& lens, const Tensor& n_new, const Tensor& block_table, const Tensor& free_pages,
+}  // namespace
+
+void fdl_torch::page_slots(const Tensor& lens, const Tensor& n_new, const Tensor& block_table, const Tensor& free_pages,
                 const Tensor& free_count, int64_t page_size, const Tensor& slots, const Tensor& positions,
                 const Tensor& cu_seqlens, const std::optional<Tensor>& new_lens,
                 const std::optional<Tensor>& new_count) {
@@ -687,6 +685,8 @@ void page_slots(const Tensor& lens, const Tensor& n_new, const Tensor& block_tab
                           new_count ? new_count->data_ptr<int32_t>() : free_count.data_ptr<int32_t>(), cur_stream()),
            "page_slots");
 }
+
+namespace {
 
 void page_release(const Tensor& done, const Tensor& lens, const Tensor& block_table, const Tensor& free_pages,
                   const Tensor& free_count, int64_t page_size) {
@@ -715,7 +715,9 @@ void check_pages(const Tensor& k, const Tensor& v, const Tensor& like, const cha
               like.dtype(), " on ", like.device(), ", contiguous in D");
 }
 
-void norm_rope_store(const Tensor& y, const Tensor& positions, const Tensor& inv_freq,
+}  // namespace
+
+void fdl_torch::norm_rope_store(const Tensor& y, const Tensor& positions, const Tensor& inv_freq,
                      const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight, double eps,
                      bool interleaved, double rope_scale, const Tensor& q, const Tensor& k_pages,
                      const Tensor& v_pages, const Tensor& slots) {
@@ -750,7 +752,7 @@ void norm_rope_store(const Tensor& y, const Tensor& positions, const Tensor& inv
            "norm_rope_store");
 }
 
-void paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
+void fdl_torch::paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& block_table,
                        const Tensor& lens, double scale, const Tensor& out) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.stride(2) == 1,
               "fdl.paged_decode_attn: q must be a CUDA [B, hq, D] tensor, contiguous in D");
@@ -784,8 +786,7 @@ void paged_decode_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
 // [rows, top]) from torch's caching allocator: a tensor each, or (`one`) four
 // parts of one allocation, which the outputs of a dispatched operator may not
 // be.
-using Scores = std::tuple<Tensor, Tensor, Tensor, Tensor>;
-Scores token_logprobs_in(const Tensor& logits, const Tensor& targets, int64_t top, bool one) {
+fdl_torch::Scores fdl_torch::token_logprobs(const Tensor& logits, const Tensor& targets, int64_t top, bool one) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
               "fdl.token_logprobs: logits must be a CUDA [rows, vocab] tensor with unit inner stride");
   const int64_t rows = logits.size(0), V = logits.size(1);
@@ -819,8 +820,13 @@ Scores token_logprobs_in(const Tensor& logits, const Tensor& targets, int64_t to
            "token_logprobs");
   return {logprob, entropy, top_lp, top_tok};
 }
+
+namespace {
+
+using fdl_torch::Scores;
+
 Scores token_logprobs(const Tensor& logits, const Tensor& targets, int64_t top) {
-  return token_logprobs_in(logits, targets, top, false);
+  return fdl_torch::token_logprobs(logits, targets, top, false);
 }
 
 Scores token_logprobs_meta(const Tensor& logits, const Tensor&, int64_t top) {
@@ -852,123 +858,6 @@ Tensor flash_kvcache(const Tensor& q, const Tensor& k_cache, const Tensor& v_cac
 Tensor flash_kvcache_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, double, bool) {
   return at::empty_like(q, q.options().memory_format(at::MemoryFormat::Contiguous));
 }
-
-// ---------------------------------------------------------------- direct calls
-// The paged-cache and scoring operators for calls of a few microseconds, where
-// the dispatcher's boxing of a dozen arguments is a third of the call: the same
-// functions that are registered below, taken from Python without it.  Only
-// plain CUDA tensors outside any dispatch mode go this way; for everything else
-// (subclasses, wrapped or fake tensors, tracing) the entry returns
-// NotImplemented and the caller uses torch.ops.fdl.
-constexpr c10::DispatchKeySet kPlainKeys =
-    c10::DispatchKeySet({c10::DispatchKey::CUDA, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutogradCUDA,
-                         c10::DispatchKey::AutocastCUDA});
-
-bool plain(PyObject* o) {
-  if (!THPVariable_CheckExact(o)) return false;
-  const auto keys = THPVariable_Unpack(o).key_set();
-  // (the difference of two sets keeps its backend bits)
-  return keys.has(c10::DispatchKey::CUDA) && ((keys - kPlainKeys).raw_repr() & ~c10::full_backend_mask) == 0;
-}
-bool plain_or_none(PyObject* o) { return o == Py_None || plain(o); }
-const Tensor& tensor(PyObject* o) { return THPVariable_Unpack(o); }
-std::optional<Tensor> maybe(PyObject* o) {
-  if (o == Py_None) return std::nullopt;
-  return THPVariable_Unpack(o);
-}
-int64_t integer(PyObject* o) {
-  const long long v = PyLong_AsLongLong(o);
-  if (v == -1 && PyErr_Occurred()) throw python_error();
-  return v;
-}
-double number(PyObject* o) {
-  const double v = PyFloat_AsDouble(o);
-  if (v == -1.0 && PyErr_Occurred()) throw python_error();
-  return v;
-}
-bool direct(PyObject* const* a, Py_ssize_t n, Py_ssize_t want, std::initializer_list<int> tensors,
-            std::initializer_list<int> optional = {}) {
-  if (n != want || c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
-  for (int i : tensors)
-    if (!plain(a[i])) return false;
-  for (int i : optional)
-    if (!plain_or_none(a[i])) return false;
-  return true;
-}
-struct NoGil {
-  PyThreadState* s = PyEval_SaveThread();
-  ~NoGil() { PyEval_RestoreThread(s); }
-};
-
-PyObject* py_page_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (!direct(a, n, 11, {0, 1, 2, 3, 4, 6, 7, 8}, {9, 10})) Py_RETURN_NOTIMPLEMENTED;
-  const Tensor lens = tensor(a[0]), n_new = tensor(a[1]), table = tensor(a[2]), pages = tensor(a[3]),
-               count = tensor(a[4]), slots = tensor(a[6]), pos = tensor(a[7]), cu = tensor(a[8]);
-  const int64_t page = integer(a[5]);
-  const auto nl = maybe(a[9]), nc = maybe(a[10]);
-  {
-    NoGil g;
-    page_slots(lens, n_new, table, pages, count, page, slots, pos, cu, nl, nc);
-  }
-  Py_RETURN_NONE;
-  END_HANDLE_TH_ERRORS
-}
-
-PyObject* py_norm_rope_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (!direct(a, n, 12, {0, 1, 2, 8, 9, 10, 11}, {3, 4})) Py_RETURN_NOTIMPLEMENTED;
-  const Tensor y = tensor(a[0]), pos = tensor(a[1]), freq = tensor(a[2]), q = tensor(a[8]), k = tensor(a[9]),
-               v = tensor(a[10]), slots = tensor(a[11]);
-  const auto qw = maybe(a[3]), kw = maybe(a[4]);
-  const double eps = number(a[5]), scale = number(a[7]);
-  const int inter = PyObject_IsTrue(a[6]);
-  if (inter < 0) throw python_error();
-  {
-    NoGil g;
-    norm_rope_store(y, pos, freq, qw, kw, eps, inter != 0, scale, q, k, v, slots);
-  }
-  Py_RETURN_NONE;
-  END_HANDLE_TH_ERRORS
-}
-
-PyObject* py_paged_decode_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (!direct(a, n, 7, {0, 1, 2, 3, 4, 6})) Py_RETURN_NOTIMPLEMENTED;
-  const Tensor q = tensor(a[0]), k = tensor(a[1]), v = tensor(a[2]), table = tensor(a[3]), lens = tensor(a[4]),
-               out = tensor(a[6]);
-  const double scale = number(a[5]);
-  {
-    NoGil g;
-    paged_decode_attn(q, k, v, table, lens, scale, out);
-  }
-  Py_RETURN_NONE;
-  END_HANDLE_TH_ERRORS
-}
-
-PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (!direct(a, n, 3, {0, 1})) Py_RETURN_NOTIMPLEMENTED;
-  const Tensor logits = tensor(a[0]), targets = tensor(a[1]);
-  const int64_t top = integer(a[2]);
-  Scores r;
-  {
-    NoGil g;
-    r = token_logprobs_in(logits, targets, top, true);
-  }
-  return Py_BuildValue("(NNNN)", THPVariable_Wrap(std::get<0>(r)), THPVariable_Wrap(std::get<1>(r)),
-                       THPVariable_Wrap(std::get<2>(r)), THPVariable_Wrap(std::get<3>(r)));
-  END_HANDLE_TH_ERRORS
-}
-
-template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
-PyMethodDef method(const char* name) {
-  return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)), METH_FASTCALL, nullptr};
-}
-PyMethodDef kMethods[] = {method<py_page_slots>("page_slots"), method<py_norm_rope_store>("norm_rope_store"),
-                          method<py_paged_decode_attn>("paged_decode_attn"),
-                          method<py_token_logprobs>("token_logprobs"), {nullptr, nullptr, 0, nullptr}};
-PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "libfdl_torch", nullptr, -1, kMethods};
 
 }  // namespace
 
@@ -1031,10 +920,10 @@ TORCH_LIBRARY_IMPL(fdl, CUDA, m) {
   m.impl("swiglu", &swiglu);
   m.impl("softmax_argmax", &softmax_argmax);
   m.impl("add_rmsnorm", &add_rmsnorm);
-  m.impl("page_slots", &page_slots);
+  m.impl("page_slots", &fdl_torch::page_slots);
   m.impl("page_release", &page_release);
-  m.impl("norm_rope_store", &norm_rope_store);
-  m.impl("paged_decode_attn", &paged_decode_attn);
+  m.impl("norm_rope_store", &fdl_torch::norm_rope_store);
+  m.impl("paged_decode_attn", &fdl_torch::paged_decode_attn);
   m.impl("token_logprobs", &token_logprobs);
 }
 
@@ -1080,5 +969,3 @@ TORCH_LIBRARY_IMPL(fdl, Meta, m) {
   m.impl("add_rmsnorm", [](const Tensor&, const Tensor&, const std::optional<Tensor>&, double,
                            const std::optional<Tensor>&, const Tensor&) {});
 }
-
-PyMODINIT_FUNC PyInit_libfdl_torch(void) { return PyModule_Create(&kModule); }

@@ -1,8 +1,15 @@
 """CPU checks of the ways into the operators: compiled calls, hosts without
 Python, calls under modes and traces."""
+import os
+import shutil
 import subprocess
 import sys
 from pathlib import Path
+
+import pytest
+import torch
+
+from fast_v2_b200 import _lib
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -38,3 +45,30 @@ for call in ({calls}):
     torch._dynamo.reset()
 """)
     assert out.split("\n")[-6:-1] == ["(9, 3)", "(2, 8, 64)", "(7,)", "(7,)", "(7,)"]
+
+
+HOST = r"""
+#include <dlfcn.h>
+#include <stdio.h>
+int main(int argc, char** argv) {
+  for (int i = 1; i < argc; ++i)
+    if (!dlopen(argv[i], RTLD_NOW | RTLD_GLOBAL)) {
+      puts(dlerror());
+      return i;
+    }
+  return dlsym(RTLD_DEFAULT, "Py_IsInitialized") ? 100 : 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not installed")
+def test_a_host_without_python_loads_the_torch_operators(tmp_path):
+    """libfdl_torch.so registers torch.ops.fdl in a libtorch process that has
+    no interpreter."""
+    src, exe = tmp_path / "host.c", tmp_path / "host"
+    src.write_text(HOST)
+    subprocess.run(["gcc", "-std=gnu99", "-Wall", "-Werror", str(src), "-ldl", "-o", str(exe)], check=True)
+    torch_lib = Path(torch.__file__).parent / "lib"
+    r = subprocess.run([str(exe), str(_lib.LIB_ABI), str(_lib.LIB_TORCH)], capture_output=True, text=True, timeout=600,
+                       env=os.environ | {"LD_LIBRARY_PATH": f"{torch_lib}:{os.environ.get('LD_LIBRARY_PATH', '')}"})
+    assert r.returncode == 0, r.stdout + r.stderr
