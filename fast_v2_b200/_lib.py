@@ -125,7 +125,8 @@ def load_if_built() -> None:
 def direct():
     """The native module whose functions take plain CUDA tensors straight into
     the operators of torch.ops.fdl, or return NotImplemented where the call has
-    to go through the dispatcher (tensor subclasses, dispatch modes)."""
+    to go through the dispatcher (tensor subclasses, dispatch and function
+    modes, torch.jit.trace, the profiler)."""
     global _direct
     if _direct is None:
         ensure_ops()  # libfdl_direct.so resolves its operators from libfdl_torch.so

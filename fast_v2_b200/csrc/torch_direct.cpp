@@ -1,13 +1,17 @@
 // Python module libfdl_direct: the paged-cache and scoring operators for calls
 // of a few microseconds, where the dispatcher's boxing of a dozen arguments is
 // a third of the call: the same functions that torch_ops.cpp registers, taken
-// from Python without it.  Only plain CUDA tensors outside any dispatch mode go
-// this way; for everything else (subclasses, wrapped or fake tensors, tracing)
-// the entry returns NotImplemented and the caller uses torch.ops.fdl.  A
-// library of its own, so that libfdl_torch.so needs no interpreter.
+// from Python without it.  Only plain CUDA tensors go this way, and only while
+// nothing watches the dispatcher; for everything else (subclasses, wrapped or
+// fake tensors, dispatch and function modes, torch.jit.trace, the profiler) the
+// entry returns NotImplemented and the caller uses torch.ops.fdl.  A library
+// of its own, so that libfdl_torch.so needs no interpreter.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/record_function.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include "torch_ops.h"
@@ -42,9 +46,16 @@ double number(PyObject* o) {
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
   return v;
 }
+// A dispatch mode, a trace or a transform adds keys to the thread's own; a
+// function mode and the profiler show elsewhere.
+bool watched() {
+  const auto keys = c10::impl::tls_local_dispatch_key_set().included_;
+  return !(keys - c10::default_included_set).empty() || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+         at::impl::torch_function_mode_enabled() || at::hasCallbacks();
+}
 bool direct(PyObject* const* a, Py_ssize_t n, Py_ssize_t want, std::initializer_list<int> tensors,
             std::initializer_list<int> optional = {}) {
-  if (n != want || c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
+  if (n != want || watched()) return false;
   for (int i : tensors)
     if (!plain(a[i])) return false;
   for (int i : optional)
