@@ -26,9 +26,11 @@ constexpr c10::DispatchKeySet kPlainKeys =
 
 bool plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return false;
-  const auto keys = THPVariable_Unpack(o).key_set();
+  const Tensor& t = THPVariable_Unpack(o);
+  const auto keys = t.key_set();
   // (the difference of two sets keeps its backend bits)
-  return keys.has(c10::DispatchKey::CUDA) && ((keys - kPlainKeys).raw_repr() & ~c10::full_backend_mask) == 0;
+  return keys.has(c10::DispatchKey::CUDA) && ((keys - kPlainKeys).raw_repr() & ~c10::full_backend_mask) == 0 &&
+         !t._fw_grad(0).defined();
 }
 bool plain_or_none(PyObject* o) { return o == Py_None || plain(o); }
 const Tensor& tensor(PyObject* o) { return THPVariable_Unpack(o); }

@@ -859,6 +859,18 @@ Tensor flash_kvcache_meta(const Tensor& q, const Tensor&, const Tensor&, const T
   return at::empty_like(q, q.options().memory_format(at::MemoryFormat::Contiguous));
 }
 
+// Autograd of operators without derivatives: nothing is recorded, and a
+// forward-mode tangent, which torch's fallback would drop in silence, is
+// refused.
+void forward_only(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  for (const auto& v : torch::jit::last(*stack, op.schema().arguments().size()))
+    if (v.isTensor())
+      TORCH_CHECK(!v.toTensor()._fw_grad(0).defined(), op.schema().name(),
+                  " has no derivatives: an input carries a forward-mode tangent");
+  at::AutoDispatchBelowADInplaceOrView below;
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(fdl, m) {
@@ -925,6 +937,11 @@ TORCH_LIBRARY_IMPL(fdl, CUDA, m) {
   m.impl("norm_rope_store", &fdl_torch::norm_rope_store);
   m.impl("paged_decode_attn", &fdl_torch::paged_decode_attn);
   m.impl("token_logprobs", &token_logprobs);
+}
+
+TORCH_LIBRARY_IMPL(fdl, Autograd, m) {
+  for (const char* op : {"norm_rope_store", "paged_decode_attn", "token_logprobs"})
+    m.impl(op, torch::CppFunction::makeFromBoxedFunction<&forward_only>());
 }
 
 TORCH_LIBRARY_IMPL(fdl, Meta, m) {

@@ -14,7 +14,8 @@ One step runs
 
 Everything runs on torch's current stream and stays on the device: lengths,
 tables and the pool are read and updated by the kernels, so a step can be
-captured in a CUDA graph and replayed.  Forward only.
+captured in a CUDA graph and replayed.  Forward only: nothing is recorded for
+autograd, and inputs with forward-mode tangents are refused.
 
 :class:`PagedKVCache` keeps the buffers of a model and calls the operators.
 """

@@ -5,7 +5,8 @@ evaluation or a server's ``logprobs`` answer takes from a whole
 ``log_softmax``: the log probability of each row's target token, the entropy
 of the row's distribution and its ``top`` most likely tokens.  It stands next
 to the greedy sampler's ``fdl_softmax_argmax``; no probabilities are
-materialised.  Forward only: nothing is recorded for autograd.
+materialised.  Forward only: nothing is recorded for autograd, and logits with a
+forward-mode tangent are refused.
 """
 from __future__ import annotations
 

@@ -72,3 +72,25 @@ def test_a_host_without_python_loads_the_torch_operators(tmp_path):
     r = subprocess.run([str(exe), str(_lib.LIB_ABI), str(_lib.LIB_TORCH)], capture_output=True, text=True, timeout=600,
                        env=os.environ | {"LD_LIBRARY_PATH": f"{torch_lib}:{os.environ.get('LD_LIBRARY_PATH', '')}"})
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_derivatives_are_refused_or_not_recorded():
+    import torch.autograd.forward_ad as fwd
+
+    _lib.ensure_ops()
+    x = torch.randn(3, 10, device="meta")
+    t = torch.zeros(3, dtype=torch.int64, device="meta")
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="derivative"):
+            torch.ops.fdl.token_logprobs(fwd.make_dual(x, torch.ones_like(x)), t, 2)
+    with pytest.raises(RuntimeError, match="derivative"):
+        torch.func.jvp(lambda y: torch.ops.fdl.token_logprobs(y, t, 2)[0], (x,), (x,))
+    r = torch.ops.fdl.token_logprobs(x.clone().requires_grad_(), t, 2)
+    assert not any(o.requires_grad for o in r)  # as with plain tensors: a backward pass says so
+    q = torch.empty(2, 4, 64, dtype=torch.bfloat16, device="meta")
+    k = torch.empty(8, 16, 2, 64, dtype=torch.bfloat16, device="meta")
+    table, lens = torch.empty((2, 2), dtype=torch.int32, device="meta"), torch.empty(2, dtype=torch.int32, device="meta")
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="derivative"):
+            torch.ops.fdl.paged_decode_attn(q, k, fwd.make_dual(k, torch.ones_like(k)), table, lens, 0.1,
+                                            torch.empty_like(q))

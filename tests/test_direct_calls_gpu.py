@@ -1,7 +1,8 @@
-"""GPU tests of calls that torch watches: traces, function modes, the profiler.
-The entries for plain tensors may not pass them by."""
+"""GPU tests of calls that torch watches: traces, function modes, the profiler,
+derivatives.  The entries for plain tensors may not pass them by."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 from torch.overrides import TorchFunctionMode
 
 from fast_v2_b200 import _lib, paged, scoring
@@ -85,6 +86,17 @@ def test_the_profiler_names_the_call(name):
     assert f"fdl::{name}" in {e.key for e in prof.key_averages()}
 
 
+@pytest.mark.parametrize("name", NAMES[:3])
+def test_forward_mode_derivatives_are_refused(name):
+    f, x = _calls()[name]
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="derivative"):
+            f(fwd.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(RuntimeError, match="derivative"):
+        torch.func.jvp(f, (x,), (x,))
+    f(x)
+
+
 def test_the_plain_entry_is_taken_without_any_of_them():
     logits, targets = torch.randn(3, 99, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
     assert _lib.direct().token_logprobs(logits, targets, 2) is not NotImplemented
@@ -94,3 +106,14 @@ def test_the_plain_entry_is_taken_without_any_of_them():
         assert _lib.direct().token_logprobs(logits, targets, 2) is not NotImplemented
     with torch.autocast("cuda"):
         assert _lib.direct().token_logprobs(logits, targets, 2) is not NotImplemented
+
+
+@pytest.mark.parametrize("name", NAMES[:3])
+def test_inputs_that_want_gradients_get_none_in_any_way_of_calling(name):
+    f, x = _calls()[name]
+    want, x = f(x), x.requires_grad_()
+    assert torch.equal(f(x), want) and not f(x).requires_grad
+    got = torch.compile(f, backend="aot_eager")(x)
+    assert torch.equal(got, want) and not got.requires_grad
+    y = x * 1.0
+    assert torch.equal(f(y), want) and not f(y).requires_grad
