@@ -952,7 +952,9 @@ int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int voc
                        float* logprob, float* entropy, int top, float* top_logprob, int64_t* top_token,
                        fdl_stream_t stream) {
   if (dtype != FDL_BF16 && dtype != FDL_F16 && dtype != FDL_F32) return FDL_E_DTYPE;
-  if (rows < 0 || vocab < 1 || row_stride < 0 || top < 0 || top > kTokMaxTop || top > vocab) return FDL_E_SHAPE;
+  if (rows < 0 || vocab < 1 || row_stride < 0 || top < 0 || top > kTokMaxTop || top > vocab ||
+      rows > INT32_MAX - kTokRowWarps)  // the rows of the last CTA, past `rows` too, are 32-bit numbers
+    return FDL_E_SHAPE;
   if (rows == 0) return FDL_OK;
   if (!logits || !targets || !logprob || !entropy || (top > 0 && (!top_logprob || !top_token))) return FDL_E_NULL;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == FDL_F32 ? 4 : 2)) return FDL_E_ALIGN;

@@ -535,8 +535,8 @@ int fdl_paged_attn(const void* q, int64_t q_sb, int64_t q_sh,
  * targets int64 [rows]: below 0 means no target (logprob 0); past the
  * vocabulary gives NaN, reported as FDL_DEV_INDEX.  Logits of -inf count as
  * probability 0.  A row with a NaN or +inf, or with nothing above -inf, is no
- * distribution: NaN outputs, tokens -1, FDL_DEV_INDEX (info = row).  top <=
- * 32 and top <= vocab; the top outputs may be NULL when top is 0.  Sums in
+ * distribution: NaN outputs, tokens -1, FDL_DEV_INDEX (info = row).  rows <
+ * 2^31 - 8, top <= 32 and top <= vocab; the top outputs may be NULL when top is 0.  Sums in
  * fp32.  Stands next to fdl_softmax_argmax: the log-likelihoods that the
  * reference's evaluation takes from whole log_softmax tensors.
  * ---------------------------------------------------------------------- */
