@@ -706,11 +706,15 @@ void page_release(const Tensor& done, const Tensor& lens, const Tensor& block_ta
            "page_release");
 }
 
+// The stride of a dimension; where it has one entry any number may stand there.
+int64_t step(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
 // K and V pages [num_pages, page_size, Hkv, D], one layout for both.
 void check_pages(const Tensor& k, const Tensor& v, const Tensor& like, const char* op) {
   TORCH_CHECK(k.is_cuda() && k.device() == like.device() && v.device() == like.device() && k.dim() == 4 &&
                   k.dtype() == like.dtype() && v.dtype() == like.dtype() && v.sizes() == k.sizes() &&
-                  v.strides() == k.strides() && k.stride(3) == 1,
+                  step(v, 0) == step(k, 0) && step(v, 1) == step(k, 1) && step(v, 2) == step(k, 2) &&
+                  v.stride(3) == 1 && k.stride(3) == 1,
               "fdl.", op, ": k_pages and v_pages must be [num_pages, page_size, Hkv, D] tensors of one layout, of ",
               like.dtype(), " on ", like.device(), ", contiguous in D");
 }
@@ -745,8 +749,8 @@ void fdl_torch::norm_rope_store(const Tensor& y, const Tensor& positions, const 
                                inv_freq.data_ptr<float>(), as_int(inv_freq.numel(), "inv_freq"),
                                q_weight ? q_weight->data_ptr() : nullptr, k_weight ? k_weight->data_ptr() : nullptr,
                                static_cast<float>(eps), interleaved, static_cast<float>(rope_scale), q.data_ptr(),
-                               k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
-                               k_pages.stride(2), as_int(k_pages.size(0), "num_pages"),
+                               k_pages.data_ptr(), v_pages.data_ptr(), step(k_pages, 0), step(k_pages, 1),
+                               step(k_pages, 2), as_int(k_pages.size(0), "num_pages"),
                                as_int(k_pages.size(1), "page_size"), slots.data_ptr<int64_t>(), rows,
                                as_int(hq, "hq"), as_int(hkv, "hkv"), as_int(D, "D"), dtype_code(y), cur_stream()),
            "norm_rope_store");
@@ -772,12 +776,12 @@ void fdl_torch::paged_decode_attn(const Tensor& q, const Tensor& k_pages, const 
                                                           block_table.size(1) * page);
   Tensor ws;
   if (ws_bytes > 0) ws = at::detail::empty_cuda({ws_bytes}, at::kByte, q.device(), std::nullopt);
-  check_rc(fdl_paged_attn(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
-                          k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), as_int(k_pages.size(0), "num_pages"),
+  check_rc(fdl_paged_attn(q.data_ptr(), step(q, 0), step(q, 1), k_pages.data_ptr(), v_pages.data_ptr(),
+                          step(k_pages, 0), step(k_pages, 1), step(k_pages, 2), as_int(k_pages.size(0), "num_pages"),
                           as_int(page, "page_size"), block_table.data_ptr<int32_t>(), table_stride(block_table),
                           as_int(block_table.size(1), "max_pages"), lens.data_ptr<int32_t>(), static_cast<int>(B),
                           static_cast<int>(hq), static_cast<int>(hkv), static_cast<int>(D), dtype_code(q),
-                          static_cast<float>(scale), out.data_ptr(), out.stride(0), out.stride(1),
+                          static_cast<float>(scale), out.data_ptr(), step(out, 0), step(out, 1),
                           ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, cur_stream()),
            "paged_decode_attn");
 }
@@ -787,7 +791,7 @@ void fdl_torch::paged_decode_attn(const Tensor& q, const Tensor& k_pages, const 
 // parts of one allocation, which the outputs of a dispatched operator may not
 // be.
 fdl_torch::Scores fdl_torch::token_logprobs(const Tensor& logits, const Tensor& targets, int64_t top, bool one) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
               "fdl.token_logprobs: logits must be a CUDA [rows, vocab] tensor with unit inner stride");
   const int64_t rows = logits.size(0), V = logits.size(1);
   check_i64(targets, logits, rows, "targets");
