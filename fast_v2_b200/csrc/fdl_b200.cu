@@ -81,18 +81,18 @@ PagedPlan paged_plan(int batch, int hq, int hkv, int head_dim, int64_t cap) {
   const int64_t units = static_cast<int64_t>(batch) * hkv * ((G + 8 * p.nh - 1) / (8 * p.nh));
   // Clusters of up to 8 CTAs of 8 warps while they fit the GPU side by side;
   // with more units, one CTA of 4 warps each.  A cluster's time follows its
-  // own sequence (0.7 us a tile and CTA), so a batch in which one sequence is
+  // own sequence (0.75 us a tile and CTA), so a batch in which one sequence is
   // long waits for it; the line costs a scan and a second kernel, but shares
-  // any batch out evenly and uses every SM.  Measured on B200, 28 query / 4 KV
-  // heads of 128, cluster against line: 320 keys B=1 5.4 / 6.0 us, B=30 6.0 /
-  // 10.2 us; 1024 keys B=16 9.0 / 10.9 us; 4096 keys B=8 16.4 / 20.2 us; 8192
-  // keys B=1 (32 CTAs) 12.2 / 10.5 us; B=100 of 1 to 1024 keys 22.7 / 27.0 us,
-  // of 1 to 4096 keys 76.7 / 72.6 us.  The limits keep the worst case, one long
+  // any batch out evenly and uses every SM.  Measured on B200, bf16, 28 query / 4
+  // KV heads of 128, cluster against line: 320 keys B=1 5.4 / 6.3 us, B=30 6.0 /
+  // 10.3 us; 1024 keys B=16 9.3 / 10.9 us; 4096 keys B=8 16.6 / 20.3 us; 8192
+  // keys B=1 (32 CTAs) 12.6 / 10.6 us; B=100 of 1 to 1024 keys 23.3 / 27.2 us,
+  // of 1 to 4096 keys 79.6 / 72.9 us.  The limits keep the worst case, one long
   // sequence among short ones, at about twice the line's time.
   // Very many short units take fewer warps each, so that more of them run at
-  // once: 1140 units of up to 36 keys 8.3 / 6.3 / 5.6 us with 4 / 2 / 1 warps,
-  // 1000 of up to 16 keys 8.7 / 6.6 / 5.2, 600 of up to 60 5.9 / 4.6 / 5.4, 800 of
-  // up to 128 9.3 / 7.6 / 9.9, of up to 256 14.6 / 13.5 / 17.1.
+  // once: 1140 units of up to 36 keys 9.8 / 8.0 / 7.4 us with 4 / 2 / 1 warps,
+  // 1000 of up to 16 keys 8.9 / 6.8 / 5.3, 600 of up to 60 6.8 / 5.9 / 6.3, 800 of
+  // up to 128 9.7 / 8.0 / 10.6, of up to 256 15.1 / 14.0 / 18.0.
   const bool few = units <= 128 && head_dim <= 128;
   p.nw = few ? 8 : kPagedLineWarps;
   if (head_dim <= 128 && units > 2 * num_sms() && cap <= 256) p.nw = cap <= 48 ? 1 : 2;
@@ -102,7 +102,8 @@ PagedPlan paged_plan(int batch, int hq, int hkv, int head_dim, int64_t cap) {
   const int most = !few ? 16 : units * p.cluster > 64 ? 8 : 5;  // tiles of a CTA
   if ((tiles + p.cluster - 1) / p.cluster > most) p.cluster = 0;
   // Two CTAs of 4 warps a unit while three CTAs a SM hold them all (160 units of
-  // up to 1000 keys 13.8 against 16.7 us; 240 units 17.6 / 17.5).
+  // up to 1000 keys 14.7 against 17.8 us; 240 units 16.7 / 20.1, but of 900 to
+  // 1000 keys 30.6 / 23.0).
   if (p.cluster == 1 && p.nw == 4 && head_dim <= 128 && tiles >= 8 && 2 * units <= 3 * num_sms()) p.cluster = 2;
   if (p.cluster) {
     p.grid = static_cast<int>(units * p.cluster);
@@ -963,13 +964,13 @@ int fdl_token_logprobs(const void* logits, int64_t row_stride, int rows, int voc
   const int64_t vectors = static_cast<int64_t>(vocab) * (dtype == FDL_F32 ? 4 : 2) / 16;
   // A warp a row for many short rows, half a CTA (128 threads) for many rows of
   // middle length, else a CTA of 256.  Measured on B200, warp / half / whole,
-  // top 20: 70000 rows of 125 vectors 109 / 410 / 649 us, 800 of 625 9.0 / 10.6
-  // / 12.8, 8000 of 1062 50 / 70 / 98, 700 of 1250 14.4 / 12.3 / 13.2, 5000 of
-  // 1750 59 / 46 / 60, 2000 of 4000 64 / 37 / 40, 1300 of 6000 86 / 38 / 36, 1500
-  // of 12564 141 / 68 / 58.  A cluster of CTAs a row where rows are few and
-  // long: it costs 2 us (100 rows of 625 vectors 5.5 us without, 7.5 us with)
-  // and divides 0.6 us a thousand vectors (19008 vectors, 1 / 2 / 4 / 8 CTAs: 8
-  // rows 16.0 / 12.6 / 10.1 / 9.2 us, 64 rows 16.5 / 13.6 / 12.2 / 14.8 us).
+  // top 20: 70000 rows of 125 vectors 109 / 361 / 600 us, 800 of 625 9.0 / 8.9 /
+  // 10.6, 8000 of 1062 50 / 62 / 91, 700 of 1250 14.4 / 10.4 / 11.7, 5000 of 1750
+  // 59 / 42 / 57, 2000 of 4000 64 / 34 / 38, 1300 of 6000 86 / 34 / 33, 1500 of
+  // 12564 140 / 62 / 57.  A cluster of CTAs a row where rows are few and long: it
+  // costs 2 us (100 rows of 625 vectors 5.0 us without, 7.1 us with) and divides
+  // 0.6 us a thousand vectors (19008 vectors, 1 / 2 / 4 / 8 CTAs: 8 rows 15.8 /
+  // 12.4 / 9.9 / 9.1 us, 64 rows 16.5 / 13.1 / 11.9 / 14.5 us).
   auto go = [&](auto t) -> int {
     using T = decltype(t);
     constexpr int kRing = kTokStages * kTokUnroll * kTokCta * 16;

@@ -83,10 +83,10 @@ constexpr float kPagedFar = 12.f;
 constexpr float kPagedDepth = 40.f;
 
 // Stages of a warp's ring.  On the line two CTAs a SM (D = 128) with three
-// stages keep HBM busy (30.7 us for 65k keys against 31.7 us with three CTAs
+// stages keep HBM busy (30.9 us for 65k keys against 31.4 us with three CTAs
 // of two stages); CTAs with a unit of their own wait on their own arithmetic,
-// and more of them with two stages win (200 rows of 1 to 1000 keys 21.8
-// against 25.1 us).
+// and more of them with two stages win (200 rows of 1 to 1000 keys 22.8
+// against 26.4 us).
 template <int D, int NW, bool LINE>
 struct PagedCfg {
   static constexpr int kStages = !LINE && (NW <= 2 || (NW == 4 && D == 128)) ? 2 : 3;

@@ -16,7 +16,9 @@
 // passes it by kTokSlack) and remembers the largest logit it saw and where.
 // The sums are kept for powers of two, 2^(x log2 e - ref'), one fused
 // multiply-add an entry; ref' is the rounded ref * log2 e, and what the
-// rounding is off is known exactly and put right at the end.
+// rounding is off is known exactly and put right at the end.  The power is the
+// hardware's, off by about two steps of fp32: the results are 9.4e-8 from 64
+// bits (512 rows of 152064; exp in full fp32 5.9e-8).
 //
 // The top k need no second pass over the row.  Order all entries by (logit,
 // lower index first).  If there are k threads whose largest entry is at or
@@ -30,9 +32,9 @@
 // entries above tau (long runs of equal logits, say) overflow the list; the
 // k-th best of the entries caught is then a better tau.
 //
-// Measured: 512 rows of 152064 bf16 logits, top 20, 38 us (4.1 TB/s; 34 us
+// Measured: 512 rows of 152064 bf16 logits, top 20, 38 us (4.1 TB/s; 32 us
 // without the top), 1500 rows of 50257 fp32, top 5, 52 us (5.8 TB/s), 8 rows of
-// 152064 9.0 us.
+// 152064 8.9 us.
 #pragma once
 #include <type_traits>
 
