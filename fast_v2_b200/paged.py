@@ -66,7 +66,9 @@ def build_slots(lens, n_new, block_table, free_pages, free_count, page_size: int
 
 def release_pages(done, lens, block_table, free_pages, free_count, page_size: int) -> None:
     """Return the pages of the sequences with ``done[b]`` (bool [B]) to the
-    pool; their table entries become -1 and their lengths 0."""
+    pool; their table entries become -1 and their lengths 0.  The pool counts no
+    owners: a page that stands in the table rows of two sequences goes back with
+    the first, and once more with the second."""
     _lib.ensure_ops()
     torch.ops.fdl.page_release(done, lens, block_table, free_pages, free_count, page_size)
 
@@ -111,7 +113,8 @@ def norm_rope_store(y, positions, inv_freq, q, k_pages, v_pages, slots, *, q_wei
     inv_freq, and write q [rows, hq, D] and the K and V rows into their slots
     of the pages [num_pages, page_size, hkv, D] (slot -1: not stored).
 
-    interleaved: pairs (2j, 2j + 1) instead of (j, j + rot / 2).  fp32
+    interleaved: pairs (2j, 2j + 1) instead of (j, j + rot / 2).  D a multiple of
+    16 up to 256, len(inv_freq) a multiple of 8.  fp32
     arithmetic, one rounding; the angle of a far position is exact (fp64).
     q may not share memory with y, nor two rows a slot.
     """
@@ -123,7 +126,8 @@ def decode_attention(q, k_pages, v_pages, block_table, lens, scale: Optional[flo
     """Attention of one query token per sequence, q [B, hq, D] (bf16 or fp16,
     D 64, 128 or 256), over the first lens[b] (int32 [B]) tokens of its pages
     [num_pages, page_size, hkv, D].  Returns [B, hq, D] (``out`` if given);
-    a sequence of length 0 gives zeros.  scale: D ** -0.5 if not given."""
+    a sequence of length 0 gives zeros.  scale: D ** -0.5 if not given.  ``out``
+    may not share memory with the inputs."""
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     _call("paged_decode_attn", q, k_pages, v_pages, block_table, lens, q.shape[-1] ** -0.5 if scale is None else scale,

@@ -37,7 +37,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0) ->
 
     Equal logits rank by index, lower first.  -inf logits are tokens of
     probability 0.  A row that is no distribution (NaN, +inf, all -inf) comes
-    out as NaN with tokens -1, and is reported in the device status.
+    out as NaN with tokens -1, and is reported in the device status.  The four
+    results share one allocation: whoever keeps one alone, or saves it, clones
+    it.
     """
     if logits.dim() != 2:
         raise ValueError(f"token_logprobs: logits must be [rows, vocab], got {tuple(logits.shape)}")

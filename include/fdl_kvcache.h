@@ -466,7 +466,8 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
  * page_size < 2^31.
  *
  * fdl_page_release: for every b with done[b] (bytes, 0 or 1) the pages of the
- * sequence go back onto the stack, its table entries become -1, its length 0.
+ * sequence go back onto the stack, its table entries become -1, its length 0
+ * (a page that two such rows name goes back twice).
  * If the stack has no room for all of them, nothing changes and
  * FDL_DEV_INDEX is reported.  The same count must not be used by another call
  * at the same time.
@@ -487,11 +488,12 @@ int fdl_softmax_argmax(const void* logits, int64_t row_stride, int rows,
  *   out[b, h] = softmax_j(scale * q[b, h] . K[b, j, h / (hq / hkv)]) V[b, j, ..]
  * over keys j < lens[b] (clamped to the table's width, FDL_DEV_LENGTH).  q and
  * out [B, hq, D] with strides; bf16 or f16, D 64, 128 or 256, hq <= 4096, any
- * hq / hkv.  A sequence without keys gives zeros.  A page outside [0, num_pages) hides its keys and
- * is reported.  Softmax in fp32; a weight enters the product as two numbers of
- * V's type.  workspace: at least
- * fdl_paged_attn_workspace_bytes() bytes, 16-byte aligned, not shared with a
- * call that may run at the same time; its contents need not be kept.
+ * hq / hkv.  A sequence without keys gives zeros.  A page outside [0,
+ * num_pages) hides its keys and is reported.  out must not overlap the inputs.
+ * Softmax in fp32; a weight enters the product as two numbers of V's type.
+ * workspace: at least fdl_paged_attn_workspace_bytes() bytes, 16-byte aligned,
+ * not shared with a call that may run at the same time; its contents need not
+ * be kept.
  * ---------------------------------------------------------------------- */
 int fdl_page_slots(const int32_t* lens, const int32_t* n_new, int batch,
                    int32_t* table, int64_t table_sb, int max_pages,
