@@ -148,3 +148,27 @@ def test_tiles_far_below_the_reference_with_infinite_scores_and_masked_pages():
     out = paged.decode_attention(q, kp, vp, table, lens, 1.0)
     assert _lib.last_device_error() == (1, -1)
     assert bool((out == 1).all())
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("gap", [9.3, 12.7, 20.1])
+def test_a_reference_that_moves_at_every_tile_does_not_drift(gap, dt):
+    """Every second run of 64 keys lies `gap` nats below the others: old and
+    new keys keep their weights through thousands of moves."""
+    B, n, D, hq, hkv = 150, 131072, 64, 4, 2
+    k = torch.zeros(1, n, hkv, D, dtype=dt, device=DEV)
+    low = (torch.arange(n, device=DEV) // 64) % 2 == 1
+    k[:, low, :, 0] = -4.0
+    k[:, 64000:64064, :, 0] = 1.0
+    v = torch.ones(1, n, hkv, D, dtype=dt, device=DEV)
+    v[:, : n // 2] = -1.0
+    v[:, :, :, D // 2:] *= torch.where(low, 16.0, 1 / 16).to(dt)[None, :, None, None]
+    q = torch.zeros(B, hq, D, dtype=dt, device=DEV)
+    q[:, :, 0] = 1.0
+    kp, vp, table = _paged(k, v, 16)
+    out = paged.decode_attention(q, kp, vp, table.repeat(B, 1), torch.full((B,), n, dtype=torch.int32, device=DEV),
+                                 gap / 4.0)
+    ref, bound = _dense(q[:1], k, v, [n], gap / 4.0)
+    ratio = ((out.double() - ref).abs() / bound).max()
+    print(f"worst share of the bound {float(ratio):.3f}, worst error {float((out.double() - ref).abs().max()):.3g}")
+    R.assert_within("attention", out, ref.expand(B, hq, D), bound.expand(B, hq, D))
