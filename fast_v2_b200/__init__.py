@@ -1,6 +1,6 @@
 """fast_v2_b200 -- B200 (sm_100a) KV-cache hot path for Fast-dLLM v2 block diffusion.
 
-Native code lives in two in-tree libraries built by ``fast_v2_b200.build``:
+Native code lives in in-tree libraries built by ``fast_v2_b200.build``:
 ``libfdl_b200.so`` (the C ABI of include/fdl_kvcache.h) and ``libfdl_torch.so``
 (torch.ops.fdl registration).  Importing the package does not load them; the
 cache/attention classes do on first use and raise ImportError if they are

@@ -863,14 +863,20 @@ Tensor flash_kvcache_meta(const Tensor& q, const Tensor&, const Tensor&, const T
   return at::empty_like(q, q.options().memory_format(at::MemoryFormat::Contiguous));
 }
 
-// Autograd of operators without derivatives: nothing is recorded, and a
-// forward-mode tangent, which torch's fallback would drop in silence, is
-// refused.
+// Autograd of operators without derivatives: nothing is recorded, so that a
+// backward pass fails.  What would be dropped in silence is refused: a
+// forward-mode tangent, and an input of torch.func.grad, which takes an output
+// that is not recorded for a constant.
 void forward_only(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
   for (const auto& v : torch::jit::last(*stack, op.schema().arguments().size()))
-    if (v.isTensor())
-      TORCH_CHECK(!v.toTensor()._fw_grad(0).defined(), op.schema().name(),
+    if (v.isTensor() && v.toTensor().defined()) {
+      const Tensor& t = v.toTensor();
+      TORCH_CHECK(!t._fw_grad(0).defined(), op.schema().name(),
                   " has no derivatives: an input carries a forward-mode tangent");
+      TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad() &&
+                    t.key_set().has(c10::DispatchKey::FuncTorchGradWrapper)),
+                  op.schema().name(), " has no derivatives: an input belongs to a torch.func transform of gradients");
+    }
   at::AutoDispatchBelowADInplaceOrView below;
   op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
 }

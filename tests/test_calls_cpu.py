@@ -85,6 +85,11 @@ def test_derivatives_are_refused_or_not_recorded():
             torch.ops.fdl.token_logprobs(fwd.make_dual(x, torch.ones_like(x)), t, 2)
     with pytest.raises(RuntimeError, match="derivative"):
         torch.func.jvp(lambda y: torch.ops.fdl.token_logprobs(y, t, 2)[0], (x,), (x,))
+    with pytest.raises(RuntimeError, match="derivative"):  # it would hand out zeros
+        torch.func.grad(lambda y: torch.ops.fdl.token_logprobs(y, t, 2)[0].sum())(x)
+    assert torch.func.grad(lambda y: (y + torch.ops.fdl.token_logprobs(y.detach(), t, 2)[0][:, None]).sum())(x).shape == x.shape
+    y = torch.func.vmap(lambda y: torch.ops.fdl.token_logprobs(y, t, 2)[0])(torch.randn(2, 3, 10, device="meta"))
+    assert y.shape == (2, 3)
     r = torch.ops.fdl.token_logprobs(x.clone().requires_grad_(), t, 2)
     assert not any(o.requires_grad for o in r)  # as with plain tensors: a backward pass says so
     q = torch.empty(2, 4, 64, dtype=torch.bfloat16, device="meta")
