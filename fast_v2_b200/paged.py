@@ -127,7 +127,12 @@ def decode_attention(q, k_pages, v_pages, block_table, lens, scale: Optional[flo
     D 64, 128 or 256), over the first lens[b] (int32 [B]) tokens of its pages
     [num_pages, page_size, hkv, D].  Returns [B, hq, D] (``out`` if given);
     a sequence of length 0 gives zeros.  scale: D ** -0.5 if not given.  ``out``
-    may not share memory with the inputs."""
+    may not share memory with the inputs.
+
+    How the work is shared out follows from the table's width, not from the
+    lengths, which stay on the device: where a caller knows that they are short,
+    a slice block_table[:, :n] that covers them is faster (30 sequences of 320
+    keys 6.0 us, in a table for 32768 tokens 10.5)."""
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     _call("paged_decode_attn", q, k_pages, v_pages, block_table, lens, q.shape[-1] ** -0.5 if scale is None else scale,
