@@ -17,8 +17,8 @@
 // The sums are kept for powers of two, 2^(x log2 e - ref'), one fused
 // multiply-add an entry; ref' is the rounded ref * log2 e, and what the
 // rounding is off is known exactly and put right at the end.  The power is the
-// hardware's, off by about two steps of fp32: the results are 9.4e-8 from 64
-// bits (512 rows of 152064; exp in full fp32 5.9e-8).
+// hardware's, off by about two steps of fp32: the results are 0.9e-7 to
+// 1.3e-7 from 64 bits (512 rows of 152064; exp in full fp32 0.6e-7).
 //
 // The top k need no second pass over the row.  Order all entries by (logit,
 // lower index first).  If there are k threads whose largest entry is at or
